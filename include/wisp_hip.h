@@ -215,6 +215,53 @@ int wisp_moe_prefill_routed(const uint8_t* pool, int64_t slot_bytes, int64_t nsl
                             uint16_t* out, float* acc, void* stream);
 
 /* ---------------------------------------------------------------------------
+ * A paged K/V cache of B sequences: kc, vc [pages][hk][page][d] of dtype (WISP_DT_BF16 or WISP_DT_F16) with element
+ * strides page_stride, head_stride and row_stride (the same for both, multiples of 8; a row's d values contiguous);
+ * page a power of two >= 16; d 64, 128 or 256. Position p of sequence b is row p % page of page
+ * table[b * width + p / page] (int32). kv_len[b]: the positions that b has, its new tokens' included. Packed tokens:
+ * those of sequence b are rows [cu[b], cu[b + 1]) of q, k, v and the output (cu int32 [B + 1], ascending from 0); the
+ * j-th of n is at position kv_len[b] - n + j; rows from cu[B] on are neither read nor written. cu, kv_len and table are
+ * device memory, read when the kernels run. A page id outside [0, pages), or a position past the table, is not
+ * dereferenced: what depends on it is NaN. No reference counterpart (the reference decodes one sequence).
+ *
+ * wisp_kv_append: RMSNorm of every q and k head (q_norm_w, k_norm_w [d], or both NULL: none), rotation of the first rot
+ * elements of each (rot a multiple of 16, at most d; pairs (i, i + rot/2), or (2i, 2i + 1) with interleaved) with row p of
+ * cos and sin [cs_rows][rot] (contiguous, cs_dtype dtype or WISP_DT_F32, one value per element:
+ * out[e] = y[e] cos[e] -/+ y[partner] sin[e]), q to qo [T][hq][d], k and v to their pages. Binary32, rounded once. q, k,
+ * v: element strides between tokens (_ts) and heads (_hs), multiples of 8, 16-byte aligned. A token without a page, or
+ * whose position is negative or not below cs_rows, stores nothing and its row of qo is NaN.
+ * Returns WISP_EINVAL, WISP_EALIGN or a hipError_t as the rest.
+ * ------------------------------------------------------------------------- */
+int wisp_kv_append(const void* q, int64_t q_ts, int64_t q_hs, const void* k, int64_t k_ts, int64_t k_hs, const void* v,
+                   int64_t v_ts, int64_t v_hs, const void* q_norm_w, const void* k_norm_w, float eps, const void* cos,
+                   const void* sin, int64_t cs_rows, int rot, int cs_dtype, int interleaved, const int32_t* cu,
+                   const int32_t* kv_len, const int32_t* table, int width, int B, int64_t T, int hq, int hk, int d,
+                   int dtype, void* kc, void* vc, int64_t pages, int page, int64_t page_stride, int64_t head_stride,
+                   int64_t row_stride, void* qo, void* stream);
+
+/* Causal attention of packed tokens over the cache: out[t] [T][hq][d] = softmax(scale q[t] . k[j]) v[j] over the positions
+ * j up to t's own; head h reads K/V head h / (hq / hk). A token at a negative position attends nothing and gives zeros.
+ * scale positive and finite. ws: wisp_attn_prompt_ws_bytes(T, B, hq, hk, d, page, width) bytes, 16-byte aligned (may be
+ * NULL where that is 0). Where a sequence reads a bad page, rows at and after it are NaN, and rows up to 255 / G tokens
+ * before may be. */
+int64_t wisp_attn_prompt_ws_bytes(int64_t T, int B, int hq, int hk, int d, int page, int width);
+int wisp_attn_prompt(const void* q, int64_t q_ts, int64_t q_hs, const void* kc, const void* vc, int64_t pages, int page,
+                     int64_t page_stride, int64_t head_stride, int64_t row_stride, const int32_t* cu, const int32_t* kv_len,
+                     const int32_t* table, int width, int B, int64_t T, int hq, int hk, int d, int dtype, float scale,
+                     void* ws, void* out, void* stream);
+
+/* One token of each sequence: out [B][hq][d] over the kv_len[b] positions of b (none: zeros). With prefix_width > 0 every
+ * sequence first attends the prefix_len[0] positions of prefix_table [prefix_width] (device int32), read once for all of
+ * them; kv_len and table are then what each sequence has of its own. ws: wisp_attn_batch_ws_bytes(B, hq, hk, d, page,
+ * prefix_width) bytes, 16-byte aligned. */
+int64_t wisp_attn_batch_ws_bytes(int B, int hq, int hk, int d, int page, int prefix_width);
+int wisp_attn_batch(const void* q, int64_t q_ts, int64_t q_hs, const void* kc, const void* vc, int64_t pages, int page,
+                    int64_t page_stride, int64_t head_stride, int64_t row_stride, const int32_t* kv_len,
+                    const int32_t* table, int width, const int32_t* prefix_len, const int32_t* prefix_table,
+                    int prefix_width, int B, int hq, int hk, int d, int dtype, float scale, void* ws, void* out,
+                    void* stream);
+
+/* ---------------------------------------------------------------------------
  * Expert cache bookkeeping (host only, no device calls). Keys are
  * layer*n_experts + expert; slots [0, n_static) are the static region.
  * policy 0 = lru, 1 = wsa (decayed frequency), 2 = static. Arithmetic is

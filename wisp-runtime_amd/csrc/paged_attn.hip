@@ -1,0 +1,900 @@
+// Attention over the paged K/V cache (paged.hpp): packed prompts, one token of each of many sequences, and one token of
+// each of many sequences behind a prefix that they share.
+//
+//     o_i = sum_{j <= lim_i} softmax_j(scale q_i . k_j) v_j
+//
+// with G = Hq/Hk query heads per K/V head, q . k and all sums in binary32 from the stored 16-bit values, o rounded once.
+// A row that may attend nothing (lim_i < 0) gives zeros. One pass over the positions with a running reference m: with
+// p_j = 2^(c (s_j - m)), c = scale log2(e), the sums l = sum p_j and O = sum p_j v_j are kept, and multiplied by
+// 2^(c (m_old - m_new)) when m moves. m need not be the maximum, only near it: it follows when the maximum has passed it
+// by 2^kLazy, so that most tiles leave O alone; the result O / l is the same. Pieces of the positions give records
+// (m, l, O) that k_attn_join adds up in the same way.
+//
+// Both kernels compute S^T = K Q^T and O^T = V^T P^T on the matrix cores: a lane then owns one query row (a column), its
+// maximum and sum are a few steps in the lane, and the lane's S^T registers are the B operand of the second product as
+// they stand, provided that V^T's positions are taken in the same order, which the LDS reads do that transpose 16-bit
+// 4 x 16 blocks. K and V reach LDS by direct loads (no registers held while in flight); their rows are stored with their
+// 16-byte chunks permuted so that both kinds of read touch all banks.
+//
+//  k_attn_rows  many query rows per K/V head (prompts, shared prefix): NW waves of 32 rows, a row being (token, head of
+//               the group), so grouped heads share every K/V tile; all waves walk the same tiles of 64 positions.
+//  k_attn_flat  one query token per sequence: a wave takes the G rows of one K/V head (16 at most), and the four waves
+//               of a workgroup, each with a slot of its own, every fourth 32 positions. HBM-bound.
+#include <math.h>
+
+#include "paged.hpp"
+#include "wisp_device.hpp"
+#include "wisp_internal.hpp"
+
+namespace wisp {
+namespace {
+
+typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
+typedef float f2_t __attribute__((ext_vector_type(2)));
+typedef short s4_t __attribute__((ext_vector_type(4)));
+typedef float f4_t __attribute__((ext_vector_type(4)));
+typedef float f16_t __attribute__((ext_vector_type(16)));
+typedef __attribute__((address_space(3))) s4_t lds_s4_t;
+
+constexpr int kTile = 64;          // positions per tile of k_attn_rows
+constexpr int kSub = 32;           // positions per slot of k_attn_flat
+constexpr int kStep = 4 * kSub;    // positions of a workgroup's four slots: the grain of its pieces
+constexpr float kLazy = 6.f;       // m follows the maximum past 2^kLazy
+constexpr int kPieces = 1024;      // pieces that k_attn_flat aims at over all sequences and K/V heads
+
+// float16 weights p: times 2^8, so that small ones keep their bits (the grain 2^-24 is then 2^-32 of the largest) and
+// 2^(8 + kLazy) stays below the type's 65,504. bfloat16 has binary32's range.
+template <bool F16>
+constexpr float kBiasP = F16 ? 8.f : 0.f;
+
+// D = A B + C, 32 x 32 x 16: lane l holds A[row l%32][8 (l/32) ..+7], B[8 (l/32) ..+7][col l%32] and, in register i,
+// D[row 8 (i/4) + 4 (l/32) + i%4][col l%32]; 16 x 16 x 32: A[row l%16][8 (l/16) ..+7], B alike, D[row 4 (l/16) + i][col l%16]
+template <bool F16>
+__device__ __forceinline__ f16_t mfma32(uint4 a, uint4 b, f16_t c) {
+    if constexpr (F16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8_t, a), __builtin_bit_cast(h8_t, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8_t, a), __builtin_bit_cast(b8_t, b), c, 0, 0, 0);
+}
+template <bool F16>
+__device__ __forceinline__ f4_t mfma16(uint4 a, uint4 b, f4_t c) {
+    if constexpr (F16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, a), __builtin_bit_cast(h8_t, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8_t, a), __builtin_bit_cast(b8_t, b), c, 0, 0, 0);
+}
+template <bool F16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    if constexpr (F16)
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2_t{lo, hi}), h2_t));
+    else
+        return pack_bf16x2(lo, hi);
+}
+template <bool F16>
+__device__ __forceinline__ float lo_of(uint32_t u) { return F16 ? half_lo_f(u) : bf16_lo(u); }
+template <bool F16>
+__device__ __forceinline__ float hi_of(uint32_t u) { return F16 ? half_hi_f(u) : bf16_hi(u); }
+
+// 4 x 16 block of 16-bit values, transposed: of each 16 lanes, lane 4r + c gives the address of row r's values 4c .. 4c+3
+// and receives column t = its number among the 16, rows 0 .. 3.
+__device__ __forceinline__ uint2 read_tr(const uint8_t* p) {
+    return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_t*)p));
+}
+
+__device__ __forceinline__ uint32_t lds_addr(const void* p) { return (uint32_t)(uintptr_t)p; }
+// 64 lanes x 16 bytes from base + each lane's 32-bit offset to LDS [lds, lds + 1024). The compiler neither emits nor counts
+// these loads: the waits for them are wait_vm<n>, n = the loads issued after the awaited ones. M0 is written here only
+// (a reserved register: the clobber is advisory), which tests/test_paged_isa.py checks.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void dma16(uint32_t lds, const uint8_t* base, uint32_t off) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds), "v"(off), "s"(base) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+template <int N>
+__device__ __forceinline__ void wait_vm() {
+    static_assert(N >= 0 && N < 64, "vmcnt is 6 bits");
+    __builtin_amdgcn_s_waitcnt((N & 15) | 0x70 | 0xF00 | ((N >> 4) << 14));
+    asm volatile("" ::: "memory");
+}
+__device__ __forceinline__ void wait_lds() {
+    __builtin_amdgcn_s_waitcnt(0xC07F);
+    asm volatile("" ::: "memory");
+}
+__device__ __forceinline__ void barrier() {
+    wait_lds();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+__device__ __forceinline__ const uint8_t* uniform(const uint8_t* p) {
+    const uint64_t v = (uint64_t)(uintptr_t)p;
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
+    return (const uint8_t*)(uintptr_t)(((uint64_t)hi << 32) | lo);
+}
+
+// Where chunk c (16 bytes) of row r is stored in its row. K is read as 16 bytes of 16 or 32 consecutive rows at one chunk:
+// rows that would share banks differ in r (two 128-byte rows cover the banks at D = 64). V is read by the transposing
+// loads, 32 lanes at a time: 4 rows x 64 bytes in k_attn_rows, 8 rows x 32 bytes in k_attn_flat.
+template <int D>
+__device__ __forceinline__ int swz_k(int r, int c) { return c ^ (D == 64 ? (r >> 1) & 7 : r & 15); }
+template <int D, bool FLAT>
+__device__ __forceinline__ int swz_v(int r, int c) {
+    if constexpr (FLAT) return c ^ (D == 64 ? ((r >> 1) & 3) << 1 : (r & 7) << 1);
+    return c ^ (D == 64 ? ((r >> 1) & 1) << 2 : (r & 3) << 2);
+}
+
+// A non-finite value in a pair: exponent bits all set.
+template <bool F16>
+__device__ __forceinline__ bool nonfinite2(uint32_t u) {
+    constexpr uint32_t M = F16 ? 0x7C00u : 0x7F80u;
+    return (u & M) == M || ((u >> 16) & M) == M;
+}
+// The values of a pair that are finite, others as 0.
+template <bool F16>
+__device__ __forceinline__ uint32_t finite2(uint32_t u) {
+    constexpr uint32_t M = F16 ? 0x7C00u : 0x7F80u;
+    return ((u & M) == M ? 0u : u & 0xFFFFu) | (((u >> 16) & M) == M ? 0u : u & 0xFFFF0000u);
+}
+
+struct RowsArgs {
+    const uint16_t* q;
+    int64_t q_ts, q_hs;  // elements
+    PagedKV kv;
+    const int *cu, *kv_len, *table;  // cu null: one sequence of B rows, none of which is masked (a shared prefix)
+    int width, B, T, hq, hk;
+    float c;        // scale * log2(e)
+    int nsplit;     // parts that the grid has for each row tile
+    int part_min;   // tiles that a part is worth
+    float *ml, *po;  // records of split row tiles: [(token * hq + head) * nsplit + part][2] and [..][D]
+    uint16_t* out;   // [T][hq][D]; null: every tile leaves records
+};
+
+struct RowTile {
+    int b, tok0, rows, r0, off, end;  // sequence, its first token, its rows, the tile's first row, position of token 0,
+                                      // positions that the tile's rows attend
+    bool bad;                         // the sequence is longer than its table
+};
+// Parts that a row tile's positions are cut into: no more than nsplit, and part_min tiles each.
+__device__ __forceinline__ int parts_of(int tiles, int nsplit, int part_min) {
+    return max(1, min(nsplit, tiles / part_min));
+}
+__device__ __forceinline__ int tile_end(int off, int rows, int r0, int bm, int G, int len) {
+    const int last = off + (min(r0 + bm, rows) - 1) / G;
+    return max(0, min(len, last + 1));
+}
+
+// Row tile number s of the pack (tiles of BM rows, sequence after sequence), or false.
+template <int BM>
+__device__ __forceinline__ bool find_tile(const RowsArgs& a, int s, int lane, RowTile& t) {
+    const int G = a.hq / a.hk;
+    t.bad = false;
+    if (!a.cu) {
+        t.b = 0, t.tok0 = 0, t.rows = a.B * G, t.r0 = s * BM;
+        t.off = 0;
+        t.end = held(a.kv_len[0], a.width, a.kv.shift, t.bad);
+        return t.r0 < t.rows;
+    }
+    int before = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 64) {
+        int lo = 0, hi = 0;
+        if (b0 + lane < a.B) token_range(a.cu, b0 + lane, a.T, lo, hi);
+        const int n = ((hi - lo) * G + BM - 1) / BM;
+        const int sum = before + wave_scan(n, lane);
+        const uint64_t mine = __ballot(s < sum);
+        if (mine) {
+            const int w = __builtin_ctzll(mine);
+            t.b = b0 + w;
+            t.tok0 = __builtin_amdgcn_readlane(lo, w);
+            const int n_tok = __builtin_amdgcn_readlane(hi, w) - t.tok0;
+            t.rows = n_tok * G;
+            t.r0 = (s - (__builtin_amdgcn_readlane(sum, w) - __builtin_amdgcn_readlane(n, w))) * BM;
+            const int len = held(a.kv_len[t.b], a.width, a.kv.shift, t.bad);
+            t.off = len - n_tok;
+            t.end = tile_end(t.off, t.rows, t.r0, BM, G, len);
+            return true;
+        }
+        before = __builtin_amdgcn_readlane(sum, 63);
+    }
+    return false;
+}
+
+// Grid: blockIdx.x = (slot * nsplit + part) * hk + head, so that a head's workgroups mostly share an XCD's L2 (hk a
+// divisor or multiple of 8); slots count down, since a prompt's last rows have the most positions.
+template <bool F16, int D, int NW>
+__global__ __launch_bounds__(64 * NW, 1) void k_attn_rows(const RowsArgs a, int slots) {
+    constexpr int BM = 32 * NW, KD = D / 16, ND = D / 32, RB = 2 * D;  // RB: bytes of a row
+    constexpr int RPI = 1024 / RB;                                      // rows per load instruction
+    constexpr int LPW = kTile / RPI / NW;                               // K (and V) load instructions per wave and tile
+    constexpr int TB = kTile * RB;
+    static_assert(kTile % (RPI * NW) == 0, "tile rows per wave");
+    __shared__ __align__(1024) uint8_t buf[2][2][TB];  // [stage][K, V]
+    __shared__ int bad_l;
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n = lane & 31, hf = lane >> 5;
+    const int G = a.hq / a.hk;
+    const int head = blockIdx.x % a.hk, rest = blockIdx.x / a.hk;
+    const int part = rest % a.nsplit, slot = slots - 1 - rest / a.nsplit;
+    RowTile t;
+    if (!find_tile<BM>(a, slot, lane, t)) return;
+    const int tiles = (t.end + kTile - 1) / kTile;
+    const int parts = a.out ? parts_of(tiles, a.nsplit, a.part_min) : a.nsplit;
+    if (part >= parts) return;
+    const int j0 = (int)((int64_t)tiles * part / parts), j1 = (int)((int64_t)tiles * (part + 1) / parts);
+    if (threadIdx.x == 0) bad_l = 0;
+
+    // this lane's query row: (token, head of the group); rows past the sequence's repeat its last and are not stored
+    const int row = t.r0 + 32 * wv + n, rr = min(row, t.rows - 1);
+    const int tok = rr / G, g = rr - tok * G;
+    const int lim = a.cu ? min(t.off + tok, t.end - 1) : t.end - 1;
+    const int wrow = t.r0 + 32 * wv;
+    const bool active = wrow < t.rows;
+    const int lim_lo = a.cu ? t.off + min(wrow, t.rows - 1) / G : t.end - 1;       // the wave's first row's
+    const int lim_hi = a.cu ? t.off + min(wrow + 31, t.rows - 1) / G : t.end - 1;  // and last row's
+    uint4 qb[KD];
+    {
+        const uint16_t* qr = a.q + (int64_t)(t.tok0 + tok) * a.q_ts + (int64_t)(head * G + g) * a.q_hs + 8 * hf;
+#pragma unroll
+        for (int s = 0; s < KD; ++s) qb[s] = *reinterpret_cast<const uint4*>(qr + 16 * s);
+    }
+
+    const int* trow = a.table + (int64_t)t.b * a.width;
+    const uint8_t* kbase = a.kv.kc + head * a.kv.hs;
+    const uint8_t* vbase = a.kv.vc + head * a.kv.hs;
+    // instruction i of this wave fills rows RPI (wv + NW i) .. of the tile; lane: row lane / (RB/16), stored chunk
+    // lane % (RB/16)
+    const int dr = lane / (RB / 16), dc = lane % (RB / 16);
+    uint32_t ko[LPW], vo[LPW];
+#pragma unroll
+    for (int i = 0; i < LPW; ++i) {
+        const int r = RPI * (wv + NW * i) + dr;
+        ko[i] = (uint32_t)(dr * (int)a.kv.rs + 16 * swz_k<D>(r, dc));
+        vo[i] = (uint32_t)(dr * (int)a.kv.rs + 16 * swz_v<D, false>(r, dc));
+    }
+    bool bad = t.bad;
+    const int last_row = max(0, t.end - 1) & ~(RPI - 1);
+    auto issue = [&](int j) {
+        uint8_t* st = &buf[j & 1][0][0];
+#pragma unroll
+        for (int i = 0; i < LPW; ++i) {
+            const int r = RPI * (wv + NW * i);
+            // rows past the end repeat the last ones: their page exists
+            const int64_t off = page_offset(a.kv, trow, a.width, min(j * kTile + r, last_row), bad);
+            dma16(lds_addr(st + r * RB), uniform(kbase + off), ko[i]);
+            dma16(lds_addr(st + TB + r * RB), uniform(vbase + off), vo[i]);
+        }
+    };
+
+    // The lane's places in a tile. K: row n (a block of 32 rows further on the same chunk: swz_k sees r % 16, or r % 16 / 2),
+    // chunk 2k + hf. V: rows 4 hf + (lane % 16) / 4 (swz_v sees r % 4), dims 32 d + 16 (lane / 16 % 2) + 4 (lane % 4).
+    int kl[KD], vl[ND];
+#pragma unroll
+    for (int k = 0; k < KD; ++k) kl[k] = n * RB + 16 * swz_k<D>(n, 2 * k + hf);
+    {
+        const int r = 4 * hf + ((lane & 15) >> 2);
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+            vl[d] = r * RB + 16 * swz_v<D, false>(r, 4 * d + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) + 8 * (lane & 1);
+    }
+
+    f16_t o[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
+    float m = -INFINITY, mb = 0.f, l = 0.f;  // reference, c * m - bias (0 while m is -inf), this lane's share of the sum
+    const float c = a.c, th = kLazy / a.c;
+
+    if (j0 < j1) issue(j0);
+    for (int j = j0; j < j1; ++j) {
+        wait_vm<0>();
+        barrier();  // every wave's part of tile j is there, and nobody reads the other stage any more
+        if (j + 1 < j1) issue(j + 1);
+        const uint8_t* kt = &buf[j & 1][0][0];
+        uint8_t* vt = &buf[j & 1][1][0];
+        const int p0 = j * kTile;
+        if (p0 + kTile > t.end) {  // rows past the end: weight 0, and nothing that 0 would not erase
+            const int from = t.end - p0;
+            for (int e = from * (RB / 16) + threadIdx.x; e < kTile * (RB / 16); e += 64 * NW)
+                *reinterpret_cast<uint4*>(vt + 16 * e) = make_uint4(0, 0, 0, 0);
+            barrier();
+        }
+        if (!active || lim_hi < p0) continue;
+        const bool masked = lim_lo < p0 + kTile - 1;
+
+        f16_t s[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[u][i] = 0.f;
+#pragma unroll
+            for (int k = 0; k < KD; ++k)
+                s[u] = mfma32<F16>(*reinterpret_cast<const uint4*>(kt + kl[k] + 32 * u * RB), qb[k], s[u]);
+        }
+        if (masked) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (p0 + 32 * u + 8 * (i >> 2) + 4 * hf + (i & 3) > lim) s[u][i] = -INFINITY;
+        }
+        float mx = s[0][0];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[u][i]);
+        mx = max_xor32(mx);
+        if (__any(mx > m + th)) {
+            const float mn = fmaxf(m, mx);
+            const float nb = mn == -INFINITY ? 0.f : mn * c - kBiasP<F16>;
+            const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mb - nb);
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[d][i] *= f;
+            m = mn;
+            mb = nb;
+        }
+        uint4 pb[4];  // B operand of positions 16 ks ..: slot 8 hf + e is position 16 ks + 8 (e/4) + 4 hf + e%4
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            float p[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i], c, -mb));
+                l += p[i];
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                pb[2 * u + h] = make_uint4(pack2<F16>(p[8 * h], p[8 * h + 1]), pack2<F16>(p[8 * h + 2], p[8 * h + 3]),
+                                           pack2<F16>(p[8 * h + 4], p[8 * h + 5]), pack2<F16>(p[8 * h + 6], p[8 * h + 7]));
+        }
+        auto v_operand = [&](int d, int ks) {
+            const uint2 x = read_tr(vt + vl[d] + 16 * ks * RB), y = read_tr(vt + vl[d] + (16 * ks + 8) * RB);
+            return make_uint4(x.x, x.y, y.x, y.y);
+        };
+        if (masked) {
+            // An infinite or NaN value at a position that some of the wave's rows do not attend: weight 0 would not keep
+            // it out of them. Rare, so looked for (in the rows past the wave's first limit) and taken by itself.
+            bool odd = false;
+            for (int e = max(lim_lo + 1 - p0, 0) * (RB / 16) + lane; e < kTile * (RB / 16); e += 64) {
+                const uint4 u = *reinterpret_cast<const uint4*>(vt + 16 * e);
+                odd = odd || nonfinite2<F16>(u.x) || nonfinite2<F16>(u.y) || nonfinite2<F16>(u.z) || nonfinite2<F16>(u.w);
+            }
+            if (__any(odd)) {
+                // the finite values as ever, then each row's odd ones where the row attends them
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int ks = 0; ks < 4; ++ks) {
+                        uint4 v = v_operand(d, ks);
+                        v = make_uint4(finite2<F16>(v.x), finite2<F16>(v.y), finite2<F16>(v.z), finite2<F16>(v.w));
+                        o[d] = mfma32<F16>(v, pb[ks], o[d]);
+                        asm volatile("" ::: "memory");  // one operand at a time: registers, not speed, count here
+                    }
+#pragma unroll 1
+                for (int r = 0; r < kTile; ++r) {
+#pragma unroll
+                    for (int d = 0; d < ND; ++d)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint2 u = *reinterpret_cast<const uint2*>(vt + r * RB + 16 * swz_v<D, false>(r, 4 * d + e) + 8 * hf);
+                            if (p0 + r <= lim && (nonfinite2<F16>(u.x) || nonfinite2<F16>(u.y))) {
+                                o[d][4 * e] += lo_of<F16>(u.x) - lo_of<F16>(finite2<F16>(u.x));
+                                o[d][4 * e + 1] += hi_of<F16>(u.x) - hi_of<F16>(finite2<F16>(u.x));
+                                o[d][4 * e + 2] += lo_of<F16>(u.y) - lo_of<F16>(finite2<F16>(u.y));
+                                o[d][4 * e + 3] += hi_of<F16>(u.y) - hi_of<F16>(finite2<F16>(u.y));
+                            }
+                            asm volatile("" ::: "memory");
+                        }
+                }
+                continue;
+            }
+        }
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) o[d] = mfma32<F16>(v_operand(d, ks), pb[ks], o[d]);
+    }
+
+    if (bad) bad_l = 1;  // any wave's
+    barrier();
+    if (!active) return;
+    l = add_xor32(l);
+    const bool poison = bad_l != 0;
+    if (row >= t.rows) return;
+    const int64_t orow = (int64_t)(t.tok0 + tok) * a.hq + head * G + g;
+    if (a.out && parts == 1) {
+        const float inv = poison ? __int_as_float(0x7FC00000) : l == 0.f ? 0.f : 1.f / l;
+        uint16_t* dst = a.out + orow * D + 4 * hf;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                *reinterpret_cast<uint2*>(dst + 32 * d + 8 * e) =
+                    make_uint2(pack2<F16>(o[d][4 * e] * inv, o[d][4 * e + 1] * inv),
+                               pack2<F16>(o[d][4 * e + 2] * inv, o[d][4 * e + 3] * inv));
+    } else {
+        const int64_t rec = orow * a.nsplit + part;
+        if (hf == 0) {
+            a.ml[2 * rec] = m;
+            a.ml[2 * rec + 1] = poison ? __int_as_float(0x7FC00000) : l;
+        }
+        float* dst = a.po + rec * D + 4 * hf;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                *reinterpret_cast<f4_t*>(dst + 32 * d + 8 * e) = f4_t{o[d][4 * e], o[d][4 * e + 1], o[d][4 * e + 2], o[d][4 * e + 3]};
+    }
+}
+
+// ---------------------------------------------------------------------------
+struct FlatArgs {
+    const uint16_t* q;
+    int64_t q_ts, q_hs;
+    PagedKV kv;
+    const int *kv_len, *table;
+    int width, B, hq, hk;
+    float c;
+    int* first;      // [B][2]: number of the sequence's first piece, its pieces
+    float *ml, *po;  // records [(first + piece) * hq + head]
+    uint16_t* out;   // [B][hq][D]; null: every piece leaves a record (a prefix's are to be added)
+};
+
+// Steps of kStep positions that a sequence needs, and the grain of the pieces: the same for every sequence, so that all
+// pieces are of like size however different the lengths are, and about kPieces of them over the K/V heads.
+__device__ __forceinline__ int steps_of(const FlatArgs& a, int b) {
+    bool over = false;
+    return b < a.B ? (held(a.kv_len[b], a.width, a.kv.shift, over) + kStep - 1) / kStep : 0;
+}
+__device__ __forceinline__ int piece_steps(const FlatArgs& a, int lane, int heads) {
+    int sum = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 64) sum += __builtin_amdgcn_readlane(wave_scan(steps_of(a, b0 + lane), lane), 63);
+    const int want = max(1, kPieces / heads);
+    return max(1, (sum + want - 1) / want);
+}
+
+template <bool F16, int D>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_flat(const FlatArgs a) {
+    constexpr int RB = 2 * D, RPI = 1024 / RB, LI = kSub / RPI, KD = D / 32, ND = D / 16;
+    constexpr int SB = kSub * RB;
+    constexpr int OS = D + 4;  // floats between rows of the join
+    __shared__ __align__(1024) uint8_t slot[4][2][SB];
+    __shared__ float red[4][16][2];
+    static_assert(sizeof(float) * 4 * 16 * OS <= sizeof(slot), "the join reuses the slots");
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n = lane & 15, r = lane >> 4;
+    const int G = a.hq / a.hk, RT = (G + 15) / 16;
+    const int hr = blockIdx.x % (a.hk * RT), head = hr % a.hk, g0 = 16 * (hr / a.hk);
+    const int id = blockIdx.x / (a.hk * RT);
+
+    // the sequence and piece of this workgroup
+    const int grain = piece_steps(a, lane, a.hk * RT);
+    int b = -1, piece = 0, pieces = 0, before = 0, len = 0;
+    for (int b0 = 0; b0 < a.B && b < 0; b0 += 64) {
+        const int np = (steps_of(a, b0 + lane) + grain - 1) / grain;
+        const int sum = before + wave_scan(np, lane);
+        const uint64_t mine = __ballot(id < sum);
+        if (mine) {
+            const int w = __builtin_ctzll(mine);
+            b = b0 + w;
+            pieces = __builtin_amdgcn_readlane(np, w);
+            before = __builtin_amdgcn_readlane(sum, w) - pieces;
+            piece = id - before;
+        } else {
+            before = __builtin_amdgcn_readlane(sum, 63);
+        }
+    }
+    if (b < 0) return;
+    bool bad = false;
+    len = held(a.kv_len[b], a.width, a.kv.shift, bad);
+    if (piece == 0 && hr == 0 && threadIdx.x == 0) {
+        a.first[2 * b] = before;
+        a.first[2 * b + 1] = pieces;
+    }
+    const int from = piece * grain * kStep, to = min(len, from + grain * kStep);
+
+    const int* trow = a.table + (int64_t)b * a.width;
+    const uint8_t* kbase = a.kv.kc + head * a.kv.hs;
+    const uint8_t* vbase = a.kv.vc + head * a.kv.hs;
+    uint8_t *ks = &slot[wv][0][0], *vs = &slot[wv][1][0];
+    const int dr = lane / (RB / 16), dc = lane % (RB / 16);
+    const int last_row = (to - 1) & ~(RPI - 1);
+    auto issue = [&](int p, bool v) {
+#pragma unroll
+        for (int i = 0; i < LI; ++i) {
+            const int rr = RPI * i + dr;
+            const int64_t off = page_offset(a.kv, trow, a.width, min(p + RPI * i, last_row), bad);
+            const uint32_t lo = (uint32_t)(dr * (int)a.kv.rs + 16 * (v ? swz_v<D, true>(rr, dc) : swz_k<D>(rr, dc)));
+            dma16(lds_addr((v ? vs : ks) + 1024 * i), uniform((v ? vbase : kbase) + off), lo);
+        }
+    };
+    const int p_first = from + kSub * wv;
+    uint4 qb[KD];
+    {
+        const uint16_t* qr = a.q + (int64_t)b * a.q_ts + (int64_t)(head * G + min(g0 + n, G - 1)) * a.q_hs + 8 * r;
+#pragma unroll
+        for (int k = 0; k < KD; ++k) qb[k] = *reinterpret_cast<const uint4*>(qr + 32 * k);
+    }
+    // the compiler's own loads are complete before the first counted one
+#pragma unroll
+    for (int k = 0; k < KD; ++k) asm volatile("" : "+v"(qb[k].x), "+v"(qb[k].y), "+v"(qb[k].z), "+v"(qb[k].w));
+    if (p_first < to) {
+        issue(p_first, false);
+        issue(p_first, true);
+    }
+
+    f4_t o[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d) o[d] = f4_t{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, mb = 0.f, l = 0.f;
+    const float c = a.c, th = kLazy / a.c;
+    for (int p = p_first; p < to; p += kStep) {
+        const bool more = p + kStep < to;
+        wait_vm<LI>();  // K is there, V may be in flight
+        f4_t s[2] = {f4_t{0.f, 0.f, 0.f, 0.f}, f4_t{0.f, 0.f, 0.f, 0.f}};
+        uint4 ka[2][KD];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int k = 0; k < KD; ++k) {
+                const int rr = 16 * u + n;
+                ka[u][k] = *reinterpret_cast<const uint4*>(ks + rr * RB + 16 * swz_k<D>(rr, 4 * k + r));
+            }
+        wait_lds();  // the K slot is read: it may be refilled
+        if (more) issue(p + kStep, false);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int k = 0; k < KD; ++k) s[u] = mfma16<F16>(ka[u][k], qb[k], s[u]);
+        if (p + kSub > to) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (p + 16 * u + 4 * r + i >= to) s[u][i] = -INFINITY;
+        }
+        float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                         fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+        mx = max_xor32(max_xor16(mx));
+        if (__any(mx > m + th)) {
+            const float mn = fmaxf(m, mx);
+            const float nb = mn == -INFINITY ? 0.f : mn * c - kBiasP<F16>;
+            const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mb - nb);
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < ND; ++d) o[d] = f4_t{o[d][0] * f, o[d][1] * f, o[d][2] * f, o[d][3] * f};
+            m = mn;
+            mb = nb;
+        }
+        // p as two terms of the type, so that its rounding costs nothing: hi + lo is p to 2^-17 of it
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            float pe[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                pe[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i], c, -mb));
+                l += pe[i];
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint32_t w = pack2<F16>(pe[2 * h], pe[2 * h + 1]);
+                hi[2 * u + h] = w;
+                lo[2 * u + h] = pack2<F16>(pe[2 * h] - lo_of<F16>(w), pe[2 * h + 1] - hi_of<F16>(w));
+            }
+        }
+        if (more) wait_vm<LI>();  // V is there, the next K may be in flight
+        else wait_vm<0>();
+        if (p + kSub > to) {  // rows past the end
+            for (int e = (to - p) * (RB / 16) + lane; e < kSub * (RB / 16); e += 64)
+                *reinterpret_cast<uint4*>(vs + 16 * e) = make_uint4(0, 0, 0, 0);
+            wait_lds();
+        }
+        uint4 va[ND];
+        const int vr = 4 * r + (n >> 2), vcn = (n & 3) >> 1, vb = 8 * (n & 1);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+            const uint2 x = read_tr(vs + vr * RB + 16 * swz_v<D, true>(vr, 2 * d + vcn) + vb);
+            const uint2 y = read_tr(vs + (vr + 16) * RB + 16 * swz_v<D, true>(vr + 16, 2 * d + vcn) + vb);
+            va[d] = make_uint4(x.x, x.y, y.x, y.y);
+        }
+        wait_lds();  // the V slot is read
+        if (more) issue(p + kStep, true);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) o[d] = mfma16<F16>(va[d], make_uint4(hi[0], hi[1], hi[2], hi[3]), o[d]);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) o[d] = mfma16<F16>(va[d], make_uint4(lo[0], lo[1], lo[2], lo[3]), o[d]);
+    }
+    wait_vm<0>();
+
+    // the four waves' sums: o[d][i] = O[row n][dim 16 d + 4 r + i]
+    l = add_xor32(add_xor16(l));
+    if (bad) l = __int_as_float(0x7FC00000);
+    if (r == 0) {
+        red[wv][n][0] = m;
+        red[wv][n][1] = l;
+    }
+    barrier();  // the slots are free, too
+    float M = red[0][n][0];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) M = fmaxf(M, red[w][n][0]);
+    const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - M) * c);
+    float* join = reinterpret_cast<float*>(&slot[0][0][0]);
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+        *reinterpret_cast<f4_t*>(join + (wv * 16 + n) * OS + 16 * d + 4 * r) = f4_t{o[d][0] * f, o[d][1] * f, o[d][2] * f, o[d][3] * f};
+    barrier();
+    const bool whole = a.out && pieces == 1;
+    for (int e = threadIdx.x; e < min(16, G - g0) * (D / 2); e += 256) {
+        const int row = e / (D / 2), d = 2 * (e - row * (D / 2));
+        float Mr = red[0][row][0], L = 0.f, x = 0.f, y = 0.f;
+#pragma unroll
+        for (int w = 1; w < 4; ++w) Mr = fmaxf(Mr, red[w][row][0]);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float mw = red[w][row][0], lw = red[w][row][1];
+            // (a wave without positions has m = -inf and l = 0, or NaN from a bad page)
+            L += mw == -INFINITY ? lw : lw * __builtin_amdgcn_exp2f((mw - Mr) * c);
+            x += join[(w * 16 + row) * OS + d];
+            y += join[(w * 16 + row) * OS + d + 1];
+        }
+        const int hd = head * G + g0 + row;
+        if (whole) {
+            *reinterpret_cast<uint32_t*>(a.out + ((int64_t)b * a.hq + hd) * D + d) = pack2<F16>(x / L, y / L);
+        } else {
+            const int64_t rec = (int64_t)(before + piece) * a.hq + hd;
+            if (d == 0) {
+                a.ml[2 * rec] = Mr;
+                a.ml[2 * rec + 1] = L;
+            }
+            *reinterpret_cast<float2*>(a.po + rec * D + d) = make_float2(x, y);
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// The records of a query row added up: those of its sequence's pieces (k_attn_flat) and those of its row tile's parts
+// (k_attn_rows). One workgroup of 4 waves per row of out; wave w takes every fourth record.
+struct JoinArgs {
+    const int *first, *kv_len;   // pieces of the sequences, or first null
+    const float *ml, *po;
+    const int *cu, *kv_own;      // prompt: cu and kv_len of the pack (which rows were cut, and into how many parts)
+    const float *rml, *rpo;      // parts: records [row * nsplit + part], or null
+    int nsplit, part_min, bm, B, T, hq, hk, cap, all;  // cap: positions of a table row; all: every row has nsplit parts (a shared prefix)
+    float c;
+    uint16_t* out;
+};
+
+template <bool F16, int D>
+__global__ __launch_bounds__(256) void k_attn_join(const JoinArgs a) {
+    constexpr int EPL = D / 64;
+    __shared__ float rm[4], rl[4], ro[4][D];
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t row = blockIdx.x;
+    const int tok = (int)(row / a.hq), hd = (int)(row - (int64_t)tok * a.hq);
+    int na = 0, nb = 0;
+    int64_t a0 = 0;
+    if (a.first) {
+        if (a.kv_len[tok] > 0) {
+            na = a.first[2 * tok + 1];
+            a0 = (int64_t)a.first[2 * tok] * a.hq + hd;
+        }
+        if (a.all) nb = a.nsplit;
+        else if (na == 1) return;  // stored whole
+    } else {
+        const int G = a.hq / a.hk;
+        int lo = 0, hi = a.B;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (a.cu[mid] <= tok) lo = mid;
+            else hi = mid;
+        }
+        int t0, t1;
+        token_range(a.cu, lo, a.T, t0, t1);
+        if (tok < t0 || tok >= t1) return;
+        const int rows = (t1 - t0) * G, r = (tok - t0) * G + hd % G, len = min(a.kv_own[lo], a.cap);
+        const int end = tile_end(len - (t1 - t0), rows, r / a.bm * a.bm, a.bm, G, len);
+        nb = parts_of((end + kTile - 1) / kTile, a.nsplit, a.part_min);
+        if (nb == 1) return;
+    }
+    float M = -INFINITY, L = 0.f, O[EPL];
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) O[e] = 0.f;
+    auto take = [&](const float* ml, const float* po, int64_t rec) {
+        const float m = ml[2 * rec], l = ml[2 * rec + 1];
+        const float mn = fmaxf(M, m);
+        const float fo = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((M - mn) * a.c);
+        const float fn = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - mn) * a.c);
+        L = L * (M == -INFINITY ? 1.f : fo) + (m == -INFINITY ? l : l * fn);  // (NaN of a bad page stays)
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) {
+            const float v = po[rec * D + EPL * lane + e];
+            O[e] = O[e] * fo + (m == -INFINITY ? 0.f : v * fn);
+        }
+        M = mn;
+    };
+    for (int i = wv; i < na; i += 4) take(a.ml, a.po, a0 + (int64_t)i * a.hq);
+    for (int i = wv; i < nb; i += 4) take(a.rml, a.rpo, row * a.nsplit + i);
+    if (lane == 0) rm[wv] = M, rl[wv] = L;
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) ro[wv][EPL * lane + e] = O[e];
+    __syncthreads();
+    if (threadIdx.x < D / 2) {
+        const int d = 2 * threadIdx.x;
+        const float Mx = fmaxf(fmaxf(rm[0], rm[1]), fmaxf(rm[2], rm[3]));
+        float x = 0.f, y = 0.f, Lt = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float f = rm[w] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((rm[w] - Mx) * a.c);
+            Lt += rm[w] == -INFINITY ? rl[w] : rl[w] * f;
+            x += ro[w][d] * f;
+            y += ro[w][d + 1] * f;
+        }
+        const float inv = Lt == 0.f ? 0.f : 1.f / Lt;
+        *reinterpret_cast<uint32_t*>(a.out + row * D + d) = pack2<F16>(x * inv, y * inv);
+    }
+}
+
+// ---------------------------------------------------------------------------
+constexpr int rows_of(int d) { return d == 256 ? 128 : 256; }  // query rows of a k_attn_rows workgroup
+
+template <bool F16>
+void launch_rows(const RowsArgs& a, int d, int slots, hipStream_t st) {
+    const dim3 grid((unsigned)((int64_t)slots * a.nsplit * a.hk));
+    if (d == 64) hipLaunchKernelGGL((k_attn_rows<F16, 64, 8>), grid, dim3(512), 0, st, a, slots);
+    else if (d == 128) hipLaunchKernelGGL((k_attn_rows<F16, 128, 8>), grid, dim3(512), 0, st, a, slots);
+    else hipLaunchKernelGGL((k_attn_rows<F16, 256, 4>), grid, dim3(256), 0, st, a, slots);
+}
+template <bool F16>
+void launch_flat(const FlatArgs& a, int d, unsigned grid, hipStream_t st) {
+    if (d == 64) hipLaunchKernelGGL((k_attn_flat<F16, 64>), dim3(grid), dim3(256), 0, st, a);
+    else if (d == 128) hipLaunchKernelGGL((k_attn_flat<F16, 128>), dim3(grid), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((k_attn_flat<F16, 256>), dim3(grid), dim3(256), 0, st, a);
+}
+template <bool F16>
+void launch_join(const JoinArgs& a, int d, unsigned grid, hipStream_t st) {
+    if (d == 64) hipLaunchKernelGGL((k_attn_join<F16, 64>), dim3(grid), dim3(256), 0, st, a);
+    else if (d == 128) hipLaunchKernelGGL((k_attn_join<F16, 128>), dim3(grid), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((k_attn_join<F16, 256>), dim3(grid), dim3(256), 0, st, a);
+}
+
+// Row tiles that T tokens of B sequences can have: each sequence's last may be partly empty.
+int64_t row_slots(int64_t T, int B, int G, int bm) { return (T * G + bm - 1) / bm + B - 1; }
+
+// Parts for each row tile: where the tiles alone leave CUs without work and the positions are many, enough to occupy the
+// card once (256 CUs, one workgroup each), but at least 4 tiles of positions each.
+int row_parts(int64_t groups, int64_t positions) {
+    const int64_t most = (positions + kTile - 1) / kTile / 4;
+    const int64_t want = groups < 1 ? 1 : 256 / groups;
+    return (int)(want < most ? (want < 1 ? 1 : want) : (most < 1 ? 1 : most));
+}
+
+int64_t rec_bytes(int64_t recs, int d) { return recs * (2 + d) * 4; }
+
+struct FlatWs {
+    int64_t pieces, first, ml, po, end;
+};
+FlatWs flat_ws(int B, int hq, int hk, int d) {
+    const int G = hq / hk, heads = hk * ((G + 15) / 16);
+    FlatWs w;
+    w.pieces = (kPieces / heads < 1 ? 1 : kPieces / heads) + B;
+    w.first = 0;
+    w.ml = ((int64_t)B * 8 + 15) / 16 * 16;
+    w.po = w.ml + (w.pieces * hq * 8 + 15) / 16 * 16;
+    w.end = w.po + w.pieces * hq * d * 4;
+    return w;
+}
+
+bool good_scale(float s) { return s > 0.f && s < INFINITY; }
+
+int check_q(const void* q, int64_t q_ts, int64_t q_hs, const void* out) {
+    if (!aligned(q, 16) || !aligned(out, 16) || q_ts % 8 || q_hs % 8) {
+        set_error("q, its strides and out must be 16-byte aligned");
+        return WISP_EALIGN;
+    }
+    return WISP_OK;
+}
+
+}  // namespace
+}  // namespace wisp
+
+using namespace wisp;
+
+extern "C" int64_t wisp_attn_prompt_ws_bytes(int64_t T, int B, int hq, int hk, int d, int page, int width) {
+    if (T < 0 || B < 1 || hk < 1 || hq < hk || hq % hk || d < 64 || page < 1 || width < 1) return -1;
+    const int parts = row_parts(row_slots(T, B, hq / hk, rows_of(d)) * hk, (int64_t)page * width);
+    return parts > 1 ? rec_bytes(T * hq * parts, d) : 0;
+}
+
+extern "C" int wisp_attn_prompt(const void* q, int64_t q_ts, int64_t q_hs, const void* kc, const void* vc, int64_t pages,
+                                int page, int64_t page_stride, int64_t head_stride, int64_t row_stride, const int32_t* cu,
+                                const int32_t* kv_len, const int32_t* table, int width, int B, int64_t T, int hq, int hk,
+                                int d, int dtype, float scale, void* ws, void* out, void* stream) {
+    clear_error();
+    if (int rc = check_paged(kc, vc, pages, page, page_stride, head_stride, row_stride, width, B, hq, hk, d, dtype)) return rc;
+    if (T < 0 || T * hq > (1 << 30)) return fail_inval("T * hq must be in [0, 2^30]");
+    if (!good_scale(scale)) return fail_inval("scale must be positive and finite");
+    if (T == 0) return WISP_OK;
+    if (!q || !cu || !kv_len || !table || !out) return fail_inval("null pointer");
+    if (int rc = check_q(q, q_ts, q_hs, out)) return rc;
+    const int bm = rows_of(d);
+    const int64_t slots = row_slots(T, B, hq / hk, bm);
+    const int parts = row_parts(slots * hk, (int64_t)page * width);
+    if (slots * hk * parts > 0x7FFFFFFF) return fail_inval("too many tokens for one call");
+    if (parts > 1 && !ws) return fail_inval("null workspace");
+    float* ml = (float*)ws;
+    float* po = ml ? ml + 2 * T * hq * parts : nullptr;
+    RowsArgs a{(const uint16_t*)q, q_ts, q_hs, paged_kv((void*)kc, (void*)vc, pages, page, page_stride, head_stride, row_stride),
+               cu, kv_len, table, width, B, (int)T, hq, hk, scale * 1.44269504088896340736f, parts, 4, ml, po, (uint16_t*)out};
+    hipStream_t st = (hipStream_t)stream;
+    if (dtype == WISP_DT_F16) launch_rows<true>(a, d, (int)slots, st);
+    else launch_rows<false>(a, d, (int)slots, st);
+    if (parts > 1) {
+        JoinArgs j{nullptr, nullptr, nullptr, nullptr, cu, kv_len, ml, po, parts, 4, bm, B, (int)T, hq, hk, width * page, 0, a.c, (uint16_t*)out};
+        if (dtype == WISP_DT_F16) launch_join<true>(j, d, (unsigned)(T * hq), st);
+        else launch_join<false>(j, d, (unsigned)(T * hq), st);
+    }
+    return check_launch("k_attn_rows");
+}
+
+// The parts of a shared prefix: rows of all B sequences together.
+static int prefix_parts(int B, int hq, int hk, int d, int64_t positions) {
+    const int bm = rows_of(d);
+    return row_parts((int64_t)(((int64_t)B * (hq / hk) + bm - 1) / bm) * hk, positions);
+}
+
+extern "C" int64_t wisp_attn_batch_ws_bytes(int B, int hq, int hk, int d, int page, int prefix_width) {
+    if (B < 1 || hk < 1 || hq < hk || hq % hk || d < 64 || page < 1 || prefix_width < 0) return -1;
+    const int64_t own = flat_ws(B, hq, hk, d).end;
+    return prefix_width ? own + rec_bytes((int64_t)B * hq * prefix_parts(B, hq, hk, d, (int64_t)page * prefix_width), d) : own;
+}
+
+extern "C" int wisp_attn_batch(const void* q, int64_t q_ts, int64_t q_hs, const void* kc, const void* vc, int64_t pages,
+                               int page, int64_t page_stride, int64_t head_stride, int64_t row_stride,
+                               const int32_t* kv_len, const int32_t* table, int width, const int32_t* prefix_len,
+                               const int32_t* prefix_table, int prefix_width, int B, int hq, int hk, int d, int dtype,
+                               float scale, void* ws, void* out, void* stream) {
+    clear_error();
+    if (int rc = check_paged(kc, vc, pages, page, page_stride, head_stride, row_stride, width, B, hq, hk, d, dtype)) return rc;
+    if (!good_scale(scale)) return fail_inval("scale must be positive and finite");
+    if (prefix_width < 0 || (int64_t)prefix_width * page > (1 << 30)) return fail_inval("the prefix's positions must be in [0, 2^30]");
+    if (!q || !kv_len || !table || !out || !ws || (prefix_width && (!prefix_len || !prefix_table))) return fail_inval("null pointer");
+    if (int rc = check_q(q, q_ts, q_hs, out)) return rc;
+    if (!aligned(ws, 16)) {
+        set_error("ws must be 16-byte aligned");
+        return WISP_EALIGN;
+    }
+    const FlatWs w = flat_ws(B, hq, hk, d);
+    const int64_t blocks = w.pieces * hk * ((hq / hk + 15) / 16);
+    if (blocks > 0x7FFFFFFF || (int64_t)B * hq > (1 << 30)) return fail_inval("too many sequences for one call");
+    const PagedKV kv = paged_kv((void*)kc, (void*)vc, pages, page, page_stride, head_stride, row_stride);
+    const float c = scale * 1.44269504088896340736f;
+    uint8_t* p = (uint8_t*)ws;
+    hipStream_t st = (hipStream_t)stream;
+    const bool f16 = dtype == WISP_DT_F16;
+    FlatArgs f{(const uint16_t*)q, q_ts, q_hs, kv, kv_len, table, width, B, hq, hk, c, (int*)p, (float*)(p + w.ml),
+               (float*)(p + w.po), prefix_width ? nullptr : (uint16_t*)out};
+    JoinArgs j{f.first, kv_len, f.ml, f.po, nullptr, nullptr, nullptr, nullptr, 0, 1, 1, B, B, hq, hk, 0, 0, c, (uint16_t*)out};
+    if (prefix_width) {
+        const int bm = rows_of(d), slots = (int)(((int64_t)B * (hq / hk) + bm - 1) / bm);
+        const int parts = prefix_parts(B, hq, hk, d, (int64_t)page * prefix_width);
+        float* rml = (float*)(p + w.end);
+        RowsArgs a{(const uint16_t*)q, q_ts, q_hs, kv, nullptr, prefix_len, prefix_table, prefix_width, B, B, hq, hk, c, parts, 1,
+                   rml, rml + 2 * (int64_t)B * hq * parts, nullptr};
+        if (f16) launch_rows<true>(a, d, slots, st);
+        else launch_rows<false>(a, d, slots, st);
+        j.rml = a.ml;
+        j.rpo = a.po;
+        j.nsplit = parts;
+        j.all = 1;
+    }
+    if (f16) launch_flat<true>(f, d, (unsigned)blocks, st);
+    else launch_flat<false>(f, d, (unsigned)blocks, st);
+    if (f16) launch_join<true>(j, d, (unsigned)(B * hq), st);
+    else launch_join<false>(j, d, (unsigned)(B * hq), st);
+    return check_launch("k_attn_flat");
+}

@@ -59,6 +59,15 @@ SIGNATURES = {
     "wisp_gptoss_ws_bytes": (_i64, [_i32, _i64, _i64]),
     "wisp_gptoss_decode": (_i32, [_vp, _i64, _i64, _vp, _i32, _i64, _i64, _i32, _i64, _vp, _vp, _vp, _i64,
                                   ctypes.c_float, ctypes.c_float, _vp, _vp, _vp]),
+    "wisp_kv_append": (_i32, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, ctypes.c_float, _vp, _vp, _i64,
+                              _i32, _i32, _i32, _vp, _vp, _vp, _i32, _i32, _i64, _i32, _i32, _i32, _i32, _vp, _vp, _i64,
+                              _i32, _i64, _i64, _i64, _vp, _vp]),
+    "wisp_attn_prompt_ws_bytes": (_i64, [_i64, _i32, _i32, _i32, _i32, _i32, _i32]),
+    "wisp_attn_prompt": (_i32, [_vp, _i64, _i64, _vp, _vp, _i64, _i32, _i64, _i64, _i64, _vp, _vp, _vp, _i32, _i32, _i64,
+                                _i32, _i32, _i32, _i32, ctypes.c_float, _vp, _vp, _vp]),
+    "wisp_attn_batch_ws_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32, _i32]),
+    "wisp_attn_batch": (_i32, [_vp, _i64, _i64, _vp, _vp, _i64, _i32, _i64, _i64, _i64, _vp, _vp, _i32, _vp, _vp, _i32,
+                               _i32, _i32, _i32, _i32, _i32, ctypes.c_float, _vp, _vp, _vp]),
     "wisp_core_create": (_i32, [_i64, _i32, _f64, _i64, _f64, _vp]),
     "wisp_core_destroy": (None, [_vp]),
     "wisp_core_step": (None, [_vp]),

@@ -536,3 +536,159 @@ def dl_route(logits, k, norm_topk, row, host_row=None, host_flag=None, seq=None)
     _lib.check(_lib.lib().wisp_dl_route(_lib.ptr(logits), logits.numel(), k, int(bool(norm_topk)), _lib.ptr(row),
                                         hr, hf, sq, _lib.stream(dev)), "dl_route")
     return row
+
+
+# ----------------------------------------------------------------------------- a paged K/V cache of several sequences
+_CACHE_DTYPES = {torch.bfloat16: _lib.WISP_DT_BF16, torch.float16: _lib.WISP_DT_F16}
+
+
+def _int32(t, n, what):
+    if t.dtype != torch.int32 or not t.is_contiguous():
+        raise TypeError(f"{what} must be a contiguous int32 tensor")
+    assert t.numel() == n, f"{what} must have {n} elements (got {t.numel()})"
+
+
+def _paged_cache(q, kc, vc, table, hq, what):
+    """Checks of a paged cache and its tables against q [.., hq, D]; the C entry points' cache arguments."""
+    D = q.shape[-1]
+    dt = _CACHE_DTYPES.get(q.dtype)
+    if dt is None or kc.dtype != q.dtype or vc.dtype != q.dtype:
+        raise TypeError(f"{what} takes bfloat16 or float16 of one dtype (got {q.dtype}, {kc.dtype}, {vc.dtype})")
+    assert kc.dim() == 4 and kc.shape == vc.shape and kc.shape[3] == D, "caches must be [pages, Hk, page, D]"
+    assert kc.stride(3) == 1 and kc.stride() == vc.stride(), "caches need contiguous rows and equal strides"
+    assert hq % kc.shape[1] == 0, f"{hq} query heads over {kc.shape[1]} K/V heads"
+    if table.dtype != torch.int32 or table.dim() != 2 or not table.is_contiguous():
+        raise TypeError("table must be a contiguous int32 [B, pages of a sequence] tensor")
+    cache = (_lib.ptr(kc), _lib.ptr(vc), kc.shape[0], kc.shape[2], kc.stride(0), kc.stride(1), kc.stride(2))
+    return dt, cache
+
+
+def _rows(x, what):
+    """x [T, h, D] with contiguous D: x, or a copy where its strides or address are not ones that the kernels read."""
+    assert x.dim() == 3, f"{what} must be [tokens, heads, D]"
+    if x.stride(2) != 1 or x.stride(0) % 8 or x.stride(1) % 8 or x.data_ptr() % 16:
+        x = x.contiguous()
+        if x.data_ptr() % 16:
+            x = x.clone()
+    return x
+
+
+def _out(out, shape, like):
+    if out is None:
+        return torch.empty(shape, dtype=like.dtype, device=like.device)
+    assert out.shape == shape and out.dtype == like.dtype and out.is_contiguous(), f"out must be a contiguous {shape} tensor"
+    return out
+
+
+def kv_append(q, k, v, cos, sin, cu, kv_len, table, kc, vc, q_norm_w=None, k_norm_w=None, eps=1e-6, interleaved=False,
+              qo=None):
+    """New tokens of several sequences into a paged K/V cache: head norms, rotation and the store, one launch.
+    dl_qk_rope for packed prompts and batches.
+
+    q [T, Hq, D], k and v [T, Hk, D] (bf16 or f16; views of a fused projection as they are): the tokens of sequence b are
+    rows cu[b] .. cu[b + 1] - 1 (cu int32 [B + 1] on the GPU, from 0), the last of them at position kv_len[b] - 1 (kv_len
+    int32 [B], the new tokens included). kc, vc [pages, Hk, page, D]: position p of b is row p % page of page
+    table[b, p // page] (int32). q_norm_w, k_norm_w [D]: RMSNorm weights of the heads, or None for none. cos, sin
+    [positions, R] (float32 or q's dtype, one value per rotated element): the first R elements of a head are rotated, in
+    pairs (i, i + R/2), or (2i, 2i + 1) where interleaved. float32 throughout, rounded once.
+    Returns the rotated q [T, Hq, D]; its rows from cu[B] on are left as they were (qo) or undefined."""
+    T, hq, D = q.shape
+    hk, B = kc.shape[1], table.shape[0]
+    dt, cache = _paged_cache(q, kc, vc, table, hq, "kv_append")
+    norms = [w for w in (q_norm_w, k_norm_w) if w is not None]
+    dev = _lib.require_gpu(q, k, v, cos, sin, cu, kv_len, table, kc, vc, *norms, what="kv_append")
+    assert k.shape == (T, hk, D) and v.shape == (T, hk, D) and k.dtype == v.dtype == q.dtype
+    _int32(cu, B + 1, "cu")
+    _int32(kv_len, B, "kv_len")
+    assert cos.dim() == 2 and cos.shape == sin.shape and cos.dtype == sin.dtype, "cos and sin must be [positions, R]"
+    if cos.dtype not in (q.dtype, torch.float32):
+        raise TypeError(f"cos and sin must be float32 or {q.dtype} (got {cos.dtype})")
+    assert len(norms) != 1, "q_norm_w and k_norm_w: both or neither"
+    for w in norms:
+        assert w.dtype == q.dtype and w.shape == (D,) and w.is_contiguous(), "norm weights must be [D] of q's dtype"
+    q, k, v, cos, sin = _rows(q, "q"), _rows(k, "k"), _rows(v, "v"), cos.contiguous(), sin.contiguous()
+    qo = _out(qo, (T, hq, D), q)
+    with torch.cuda.device(dev):
+        _lib.check(
+            _lib.lib().wisp_kv_append(
+                _lib.ptr(q), q.stride(0), q.stride(1), _lib.ptr(k), k.stride(0), k.stride(1), _lib.ptr(v), v.stride(0),
+                v.stride(1), _lib.ptr(q_norm_w), _lib.ptr(k_norm_w), float(eps), _lib.ptr(cos), _lib.ptr(sin),
+                cos.shape[0], cos.shape[1], _X_DTYPES[cos.dtype], int(bool(interleaved)), _lib.ptr(cu), _lib.ptr(kv_len),
+                _lib.ptr(table), table.shape[1], B, T, hq, hk, D, dt, *cache, _lib.ptr(qo), _lib.stream(dev),
+            ),
+            "kv_append",
+        )
+    return qo
+
+
+def attn_prompt(q, kc, vc, cu, kv_len, table, scale, out=None):
+    """Causal attention of packed prompts over a paged K/V cache: q [T, Hq, D] (kv_append's result), cu, kv_len, table, kc
+    and vc as kv_append takes them, the tokens' own keys and values stored before the call. A token attends the positions
+    of its sequence up to its own, cached ones included; scale > 0. Returns [T, Hq, D]; rows from cu[B] on are left as they
+    were (out) or undefined. Nothing is read back to the host, so the call can be captured and the lengths changed between
+    replays."""
+    T, hq, D = q.shape
+    hk, B = kc.shape[1], table.shape[0]
+    dt, cache = _paged_cache(q, kc, vc, table, hq, "attn_prompt")
+    dev = _lib.require_gpu(q, kc, vc, cu, kv_len, table, what="attn_prompt")
+    _int32(cu, B + 1, "cu")
+    _int32(kv_len, B, "kv_len")
+    q = _rows(q, "q")
+    out = _out(out, (T, hq, D), q)
+    L = _lib.lib()
+    nb = L.wisp_attn_prompt_ws_bytes(T, B, hq, hk, D, kc.shape[2], table.shape[1])
+    with torch.cuda.device(dev):
+        ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb > 0 else None
+        _lib.check(
+            L.wisp_attn_prompt(
+                _lib.ptr(q), q.stride(0), q.stride(1), *cache, _lib.ptr(cu), _lib.ptr(kv_len), _lib.ptr(table),
+                table.shape[1], B, T, hq, hk, D, dt, float(scale), _lib.ptr(ws), _lib.ptr(out), _lib.stream(dev),
+            ),
+            "attn_prompt",
+        )
+    return out
+
+
+def _attn_batch(q, kc, vc, kv_len, table, prefix_len, prefix_table, scale, out, what):
+    B, hq, D = q.shape
+    hk = kc.shape[1]
+    dt, cache = _paged_cache(q, kc, vc, table, hq, what)
+    assert table.shape[0] == B, f"{B} rows of q, {table.shape[0]} of table"
+    pre = [t for t in (prefix_len, prefix_table) if t is not None]
+    dev = _lib.require_gpu(q, kc, vc, kv_len, table, *pre, what=what)
+    _int32(kv_len, B, "kv_len")
+    width = 0
+    if pre:
+        width = prefix_table.numel()
+        _int32(prefix_len, 1, "prefix_len")
+        _int32(prefix_table, width, "prefix_table")
+        assert prefix_table.dim() == 1 and width >= 1, "prefix_table must be [pages of the prefix]"
+    q = _rows(q, "q")
+    out = _out(out, (B, hq, D), q)
+    L = _lib.lib()
+    nb = L.wisp_attn_batch_ws_bytes(B, hq, hk, D, kc.shape[2], width)
+    with torch.cuda.device(dev):
+        ws = torch.empty(max(nb, 0), dtype=torch.uint8, device=dev)
+        _lib.check(
+            L.wisp_attn_batch(
+                _lib.ptr(q), q.stride(0), q.stride(1), *cache, _lib.ptr(kv_len), _lib.ptr(table), table.shape[1],
+                _lib.ptr(prefix_len), _lib.ptr(prefix_table), width, B, hq, hk, D, dt, float(scale), _lib.ptr(ws),
+                _lib.ptr(out), _lib.stream(dev),
+            ),
+            what,
+        )
+    return out
+
+
+def attn_batch(q, kc, vc, kv_len, table, scale, out=None):
+    """attn_decode for a batch: one token of each of B sequences, q [B, Hq, D] (bf16 or f16), over the kv_len[b] positions
+    that sequence b has in the paged cache kc, vc [pages, Hk, page, D] (kv_len int32 [B] and table int32 [B, pages of a
+    sequence] on the GPU; a sequence without positions gives zeros). Returns [B, Hq, D]."""
+    return _attn_batch(q, kc, vc, kv_len, table, None, None, scale, out, "attn_batch")
+
+
+def attn_shared(q, kc, vc, kv_len, table, prefix_len, prefix_table, scale, out=None):
+    """attn_batch for sequences that begin with the same prefix: every row of q first attends the prefix_len[0] (int32 [1])
+    positions in the pages prefix_table (int32 [pages of the prefix]), whose keys and values are read once for the whole
+    batch, then its own kv_len[b] positions in table[b]."""
+    return _attn_batch(q, kc, vc, kv_len, table, prefix_len, prefix_table, scale, out, "attn_shared")
