@@ -20,6 +20,12 @@ struct PagedKV {
     int pages, shift;    // pages in the cache; log2 of the positions per page
 };
 
+// p[i] for an i that all lanes share, as a scalar load: cu, kv_len and table do not change while a kernel runs. (As a vector
+// load it would count, and be awaited, together with the direct loads to LDS that are in flight.)
+__device__ __forceinline__ int scalar_at(const int* p, int i) {
+    return *(const __attribute__((address_space(4))) int*)(uintptr_t)(p + __builtin_amdgcn_readfirstlane(i));
+}
+
 // Byte offset of position pos of the sequence whose table row is trow (width entries); bad where there is none.
 __device__ __forceinline__ int64_t page_offset(const PagedKV& kv, const int* __restrict__ trow, int width, int pos, bool& bad) {
     const int i = pos >> kv.shift;

@@ -104,9 +104,11 @@ __device__ __forceinline__ void wait_lds() {
     asm volatile("" ::: "memory");
 }
 __device__ __forceinline__ void barrier() {
+    __builtin_amdgcn_sched_barrier(0);  // arithmetic stays on its side, too
     wait_lds();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
 }
 __device__ __forceinline__ const uint8_t* uniform(const uint8_t* p) {
     const uint64_t v = (uint64_t)(uintptr_t)p;
@@ -137,6 +139,19 @@ __device__ __forceinline__ uint32_t finite2(uint32_t u) {
     constexpr uint32_t M = F16 ? 0x7C00u : 0x7F80u;
     return ((u & M) == M ? 0u : u & 0xFFFFu) | (((u >> 16) & M) == M ? 0u : u & 0xFFFF0000u);
 }
+
+// The order of a turn's LDS reads and matrix instructions: NV operands of V (two reads each), then NK of K (one read), each
+// read kAhead instructions before its use. (Left to itself the compiler reads two at a time and waits for them.)
+constexpr int kAhead = 4;
+template <int NV, int NK, int I>
+__device__ __forceinline__ void order_step() {
+    if constexpr (I >= kAhead) __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+    if constexpr (I < NV) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+    else if constexpr (I < NV + NK) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    if constexpr (I + 1 < NV + NK + kAhead) order_step<NV, NK, I + 1>();
+}
+template <int NV, int NK>
+__device__ __forceinline__ void order_turn() { order_step<NV, NK, 0>(); }
 
 struct RowsArgs {
     const uint16_t* q;
@@ -173,7 +188,7 @@ __device__ __forceinline__ bool find_tile(const RowsArgs& a, int s, int lane, Ro
     if (!a.cu) {
         t.b = 0, t.tok0 = 0, t.rows = a.B * G, t.r0 = s * BM;
         t.off = 0;
-        t.end = held(a.kv_len[0], a.width, a.kv.shift, t.bad);
+        t.end = held(scalar_at(a.kv_len, 0), a.width, a.kv.shift, t.bad);
         return t.r0 < t.rows;
     }
     int before = 0;
@@ -190,7 +205,7 @@ __device__ __forceinline__ bool find_tile(const RowsArgs& a, int s, int lane, Ro
             const int n_tok = __builtin_amdgcn_readlane(hi, w) - t.tok0;
             t.rows = n_tok * G;
             t.r0 = (s - (__builtin_amdgcn_readlane(sum, w) - __builtin_amdgcn_readlane(n, w))) * BM;
-            const int len = held(a.kv_len[t.b], a.width, a.kv.shift, t.bad);
+            const int len = held(scalar_at(a.kv_len, t.b), a.width, a.kv.shift, t.bad);
             t.off = len - n_tok;
             t.end = tile_end(t.off, t.rows, t.r0, BM, G, len);
             return true;
@@ -202,15 +217,23 @@ __device__ __forceinline__ bool find_tile(const RowsArgs& a, int s, int lane, Ro
 
 // Grid: blockIdx.x = (slot * nsplit + part) * hk + head, so that a head's workgroups mostly share an XCD's L2 (hk a
 // divisor or multiple of 8); slots count down, since a prompt's last rows have the most positions.
+//
+// A tile costs a wave 4 D / 8 matrix instructions of 32 cycles each (S and O, 1,024 cycles at D = 128) and about as many
+// VALU cycles (32 weights per lane), and the LDS reads of its operands are as long. With eight waves, two to a SIMD, the
+// two halves of the workgroup take turns: while waves 0-3 run a tile's matrix products, waves 4-7 weigh their tile, and
+// a barrier swaps the parts. A turn M(j) is O += V(j) P(j), then S(j + 1) = K(j + 1) Q^T; a turn W(j) turns S(j) into
+// P(j). K and V of four tiles are in LDS or on their way.
 template <bool F16, int D, int NW>
 __global__ __launch_bounds__(64 * NW, 1) void k_attn_rows(const RowsArgs a, int slots) {
     constexpr int BM = 32 * NW, KD = D / 16, ND = D / 32, RB = 2 * D;  // RB: bytes of a row
     constexpr int RPI = 1024 / RB;                                      // rows per load instruction
     constexpr int LPW = kTile / RPI / NW;                               // K (and V) load instructions per wave and tile
     constexpr int TB = kTile * RB;
+    constexpr bool TURNS = NW == 8;
+    constexpr int NST = TURNS ? 4 : 2;  // tiles in LDS
     static_assert(kTile % (RPI * NW) == 0, "tile rows per wave");
-    __shared__ __align__(1024) uint8_t buf[2][2][TB];  // [stage][K, V]
-    __shared__ int bad_l;
+    __shared__ __align__(1024) uint8_t buf[NST][2][TB];  // [stage][K, V]
+    __shared__ int bad_l, odd_l;  // a page that does not exist; an infinite or NaN value taken out of V
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 31, hf = lane >> 5;
     const int G = a.hq / a.hk;
@@ -222,7 +245,54 @@ __global__ __launch_bounds__(64 * NW, 1) void k_attn_rows(const RowsArgs a, int 
     const int parts = a.out ? parts_of(tiles, a.nsplit, a.part_min) : a.nsplit;
     if (part >= parts) return;
     const int j0 = (int)((int64_t)tiles * part / parts), j1 = (int)((int64_t)tiles * (part + 1) / parts);
-    if (threadIdx.x == 0) bad_l = 0;
+    if (threadIdx.x == 0) bad_l = odd_l = 0;
+
+    const int* trow = a.table + (int64_t)t.b * a.width;
+    const uint8_t* kbase = a.kv.kc + head * a.kv.hs;
+    const uint8_t* vbase = a.kv.vc + head * a.kv.hs;
+    // instruction i of this wave fills rows RPI (wv + NW i) .. of the tile; lane: row lane / (RB/16), stored chunk
+    // lane % (RB/16)
+    constexpr int SAME = RPI * NW % 16 == 0 ? 1 : LPW;  // the permutation has period 16 in the row
+    const int dr = lane / (RB / 16), dc = lane % (RB / 16);
+    uint32_t ko[SAME], vo[SAME];
+#pragma unroll
+    for (int i = 0; i < SAME; ++i) {
+        const int r = RPI * (wv + NW * i) + dr;
+        ko[i] = (uint32_t)(dr * (int)a.kv.rs + 16 * swz_k<D>(r, dc));
+        vo[i] = (uint32_t)(dr * (int)a.kv.rs + 16 * swz_v<D, false>(r, dc));
+    }
+    bool bad = t.bad;
+    const int last_row = max(0, t.end - 1) & ~(RPI - 1);
+    // Tile j's page ids, read a turn before its loads are issued (rows past the end repeat the last ones: their page exists).
+    int page[LPW];
+    auto row_of = [&](int j, int i) { return min(j * kTile + RPI * (wv + NW * i), last_row); };
+    auto find_pages = [&](int j) {
+#pragma unroll
+        for (int i = 0; i < LPW; ++i) {
+            const int at = row_of(j, i) >> a.kv.shift;
+            page[i] = scalar_at(trow, min(at, a.width - 1));
+            if (at >= a.width) page[i] = -1;
+        }
+    };
+    auto issue = [&](int j) {
+        const uint32_t st = lds_addr(&buf[j & (NST - 1)][0][0]);
+#pragma unroll
+        for (int i = 0; i < LPW; ++i) {
+            const int r = RPI * (wv + NW * i);
+            const bool ok = (unsigned)page[i] < (unsigned)a.kv.pages;
+            bad = bad || !ok;
+            const int64_t off = (ok ? (int64_t)page[i] : 0) * a.kv.ps + (int64_t)(row_of(j, i) & ((1 << a.kv.shift) - 1)) * a.kv.rs;
+            dma16(st + r * RB, uniform(kbase + off), ko[i % SAME]);
+            dma16(st + TB + r * RB, uniform(vbase + off), vo[i % SAME]);
+        }
+    };
+    const bool late = TURNS && wv >= NW / 2;
+    const int lead = late ? 3 : TURNS ? 2 : 1;  // tiles requested before the first is used
+    for (int j = j0; j < min(j1, j0 + lead); ++j) {
+        find_pages(j);
+        issue(j);
+    }
+    find_pages(j0 + lead);
 
     // this lane's query row: (token, head of the group); rows past the sequence's repeat its last and are not stored
     const int row = t.r0 + 32 * wv + n, rr = min(row, t.rows - 1);
@@ -238,33 +308,10 @@ __global__ __launch_bounds__(64 * NW, 1) void k_attn_rows(const RowsArgs a, int 
 #pragma unroll
         for (int s = 0; s < KD; ++s) qb[s] = *reinterpret_cast<const uint4*>(qr + 16 * s);
     }
-
-    const int* trow = a.table + (int64_t)t.b * a.width;
-    const uint8_t* kbase = a.kv.kc + head * a.kv.hs;
-    const uint8_t* vbase = a.kv.vc + head * a.kv.hs;
-    // instruction i of this wave fills rows RPI (wv + NW i) .. of the tile; lane: row lane / (RB/16), stored chunk
-    // lane % (RB/16)
-    const int dr = lane / (RB / 16), dc = lane % (RB / 16);
-    uint32_t ko[LPW], vo[LPW];
+    // q arrives here: awaited where it is first used, inside the loop, it would have the compiler wait there for every load
+    // in flight, each time round
 #pragma unroll
-    for (int i = 0; i < LPW; ++i) {
-        const int r = RPI * (wv + NW * i) + dr;
-        ko[i] = (uint32_t)(dr * (int)a.kv.rs + 16 * swz_k<D>(r, dc));
-        vo[i] = (uint32_t)(dr * (int)a.kv.rs + 16 * swz_v<D, false>(r, dc));
-    }
-    bool bad = t.bad;
-    const int last_row = max(0, t.end - 1) & ~(RPI - 1);
-    auto issue = [&](int j) {
-        uint8_t* st = &buf[j & 1][0][0];
-#pragma unroll
-        for (int i = 0; i < LPW; ++i) {
-            const int r = RPI * (wv + NW * i);
-            // rows past the end repeat the last ones: their page exists
-            const int64_t off = page_offset(a.kv, trow, a.width, min(j * kTile + r, last_row), bad);
-            dma16(lds_addr(st + r * RB), uniform(kbase + off), ko[i]);
-            dma16(lds_addr(st + TB + r * RB), uniform(vbase + off), vo[i]);
-        }
-    };
+    for (int k = 0; k < KD; ++k) asm volatile("" : "+v"(qb[k].x), "+v"(qb[k].y), "+v"(qb[k].z), "+v"(qb[k].w));
 
     // The lane's places in a tile. K: row n (a block of 32 rows further on the same chunk: swz_k sees r % 16, or r % 16 / 2),
     // chunk 2k + hf. V: rows 4 hf + (lane % 16) / 4 (swz_v sees r % 4), dims 32 d + 16 (lane / 16 % 2) + 4 (lane % 4).
@@ -278,41 +325,30 @@ __global__ __launch_bounds__(64 * NW, 1) void k_attn_rows(const RowsArgs a, int 
             vl[d] = r * RB + 16 * swz_v<D, false>(r, 4 * d + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) + 8 * (lane & 1);
     }
 
-    f16_t o[ND];
+    f16_t o[ND], s[2];
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
     float m = -INFINITY, mb = 0.f, l = 0.f;  // reference, c * m - bias (0 while m is -inf), this lane's share of the sum
     const float c = a.c, th = kLazy / a.c;
+    uint4 pb[4];  // B operand of positions 16 ks ..: slot 8 hf + e is position 16 ks + 8 (e/4) + 4 hf + e%4
 
-    if (j0 < j1) issue(j0);
-    for (int j = j0; j < j1; ++j) {
-        wait_vm<0>();
-        barrier();  // every wave's part of tile j is there, and nobody reads the other stage any more
-        if (j + 1 < j1) issue(j + 1);
-        const uint8_t* kt = &buf[j & 1][0][0];
-        uint8_t* vt = &buf[j & 1][1][0];
-        const int p0 = j * kTile;
-        if (p0 + kTile > t.end) {  // rows past the end: weight 0, and nothing that 0 would not erase
-            const int from = t.end - p0;
-            for (int e = from * (RB / 16) + threadIdx.x; e < kTile * (RB / 16); e += 64 * NW)
-                *reinterpret_cast<uint4*>(vt + 16 * e) = make_uint4(0, 0, 0, 0);
-            barrier();
-        }
-        if (!active || lim_hi < p0) continue;
-        const bool masked = lim_lo < p0 + kTile - 1;
-
-        f16_t s[2];
+    auto scores = [&](int j) {  // S(j)
+        const uint8_t* kt = &buf[j & (NST - 1)][0][0];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[u][i] = 0.f;
 #pragma unroll
-            for (int k = 0; k < KD; ++k)
+        for (int k = 0; k < KD; ++k)
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
                 s[u] = mfma32<F16>(*reinterpret_cast<const uint4*>(kt + kl[k] + 32 * u * RB), qb[k], s[u]);
-        }
-        if (masked) {
+    };
+    auto weigh = [&](int j) {  // P(j), m, l
+        const int p0 = j * kTile;
+        if (lim_lo < p0 + kTile - 1) {
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -337,7 +373,6 @@ __global__ __launch_bounds__(64 * NW, 1) void k_attn_rows(const RowsArgs a, int 
             m = mn;
             mb = nb;
         }
-        uint4 pb[4];  // B operand of positions 16 ks ..: slot 8 hf + e is position 16 ks + 8 (e/4) + 4 hf + e%4
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             float p[16];
@@ -351,57 +386,144 @@ __global__ __launch_bounds__(64 * NW, 1) void k_attn_rows(const RowsArgs a, int 
                 pb[2 * u + h] = make_uint4(pack2<F16>(p[8 * h], p[8 * h + 1]), pack2<F16>(p[8 * h + 2], p[8 * h + 3]),
                                            pack2<F16>(p[8 * h + 4], p[8 * h + 5]), pack2<F16>(p[8 * h + 6], p[8 * h + 7]));
         }
+        // the weights are formed here, in this turn: the compiler would move them to where they are used, past the barrier
+#pragma unroll
+        for (int k = 0; k < 4; ++k) asm volatile("" : "+v"(pb[k].x), "+v"(pb[k].y), "+v"(pb[k].z), "+v"(pb[k].w));
+    };
+    auto collect = [&](int j) {  // O += V(j) P(j)
+        const uint8_t* vt = &buf[j & (NST - 1)][1][0];
         auto v_operand = [&](int d, int ks) {
             const uint2 x = read_tr(vt + vl[d] + 16 * ks * RB), y = read_tr(vt + vl[d] + (16 * ks + 8) * RB);
             return make_uint4(x.x, x.y, y.x, y.y);
         };
-        if (masked) {
-            // An infinite or NaN value at a position that some of the wave's rows do not attend: weight 0 would not keep
-            // it out of them. Rare, so looked for (in the rows past the wave's first limit) and taken by itself.
-            bool odd = false;
-            for (int e = max(lim_lo + 1 - p0, 0) * (RB / 16) + lane; e < kTile * (RB / 16); e += 64) {
-                const uint4 u = *reinterpret_cast<const uint4*>(vt + 16 * e);
-                odd = odd || nonfinite2<F16>(u.x) || nonfinite2<F16>(u.y) || nonfinite2<F16>(u.z) || nonfinite2<F16>(u.w);
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+            for (int d = 0; d < ND; ++d) o[d] = mfma32<F16>(v_operand(d, ks), pb[ks], o[d]);
+    };
+    // Where a tile has positions that not all rows attend, V must hold nothing that weight 0 would not erase: rows past the
+    // end, which may hold anything, are cleared, and an infinite or NaN value is taken out and added at the end to those
+    // rows that attend it. By the threads first, first + many, ..
+    const int lim_wg = a.cu ? t.off + t.r0 / G : t.end - 1;  // the tile's first row's limit
+    auto unsafe = [&](int j) { return (j + 1) * kTile - 1 > lim_wg; };
+    auto make_safe = [&](int j, int first, int many) {
+        uint8_t* vt = &buf[j & (NST - 1)][1][0];
+        const int tail = (t.end - j * kTile) * (RB / 16);
+        for (int e = first; e < kTile * (RB / 16); e += many) {
+            uint4 u = e < tail ? *reinterpret_cast<const uint4*>(vt + 16 * e) : make_uint4(0, 0, 0, 0);
+            const bool odd = nonfinite2<F16>(u.x) || nonfinite2<F16>(u.y) || nonfinite2<F16>(u.z) || nonfinite2<F16>(u.w);
+            if (odd) {
+                u = make_uint4(finite2<F16>(u.x), finite2<F16>(u.y), finite2<F16>(u.z), finite2<F16>(u.w));
+                odd_l = 1;
             }
-            if (__any(odd)) {
-                // the finite values as ever, then each row's odd ones where the row attends them
-#pragma unroll
-                for (int d = 0; d < ND; ++d)
-#pragma unroll
-                    for (int ks = 0; ks < 4; ++ks) {
-                        uint4 v = v_operand(d, ks);
-                        v = make_uint4(finite2<F16>(v.x), finite2<F16>(v.y), finite2<F16>(v.z), finite2<F16>(v.w));
-                        o[d] = mfma32<F16>(v, pb[ks], o[d]);
-                        asm volatile("" ::: "memory");  // one operand at a time: registers, not speed, count here
-                    }
-#pragma unroll 1
-                for (int r = 0; r < kTile; ++r) {
-#pragma unroll
-                    for (int d = 0; d < ND; ++d)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const uint2 u = *reinterpret_cast<const uint2*>(vt + r * RB + 16 * swz_v<D, false>(r, 4 * d + e) + 8 * hf);
-                            if (p0 + r <= lim && (nonfinite2<F16>(u.x) || nonfinite2<F16>(u.y))) {
-                                o[d][4 * e] += lo_of<F16>(u.x) - lo_of<F16>(finite2<F16>(u.x));
-                                o[d][4 * e + 1] += hi_of<F16>(u.x) - hi_of<F16>(finite2<F16>(u.x));
-                                o[d][4 * e + 2] += lo_of<F16>(u.y) - lo_of<F16>(finite2<F16>(u.y));
-                                o[d][4 * e + 3] += hi_of<F16>(u.y) - hi_of<F16>(finite2<F16>(u.y));
-                            }
-                            asm volatile("" ::: "memory");
-                        }
+            if (odd || e >= tail) *reinterpret_cast<uint4*>(vt + 16 * e) = u;
+        }
+    };
+
+    if constexpr (TURNS) {
+        // Interval 2j is W(j) of waves 0-3 and M(j - 1) of waves 4-7, interval 2j + 1 the other way round. In W(j) waves 0-3
+        // request their part of tile j + 2 and waves 4-7 theirs of tile j + 3, whose stages' tiles j - 2 and j - 1 nobody
+        // reads any more. All await tile j + 1 before interval 2j + 1, that of M(j), which is the first to read it, with one
+        // tile after it still on its way.
+        auto await = [&](bool newer) {
+            if (newer) wait_vm<2 * LPW>();
+            else wait_vm<0>();
+        };
+        if (j0 < j1) {
+            await(false);
+            barrier();
+            if (late) {
+                await(j0 + 2 < j1);  // tile j0 + 1
+                barrier();
+            }
+            // the wave's own tiles are j0 .. jw - 1: past them its rows attend nothing
+            const int jw = active && lim_hi >= j0 * kTile ? min(j1, lim_hi / kTile + 1) : j0;
+            auto begin_w = [&](int j) {
+                if (j + lead < j1) {
+                    issue(j + lead);
+                    find_pages(j + lead + 1);
                 }
-                continue;
+                if (!late && unsafe(j)) make_safe(j, threadIdx.x, 32 * NW);
+            };
+            auto end_w = [&](int j) {
+                if (!late) await(j + 2 < j1);  // tile j + 1
+                barrier();
+            };
+            auto end_m = [&](int j) {
+                if (late) await(j + 3 < j1);  // tile j + 2
+                barrier();
+            };
+            if (j0 < jw) {
+                scores(j0);
+                order_turn<0, 2 * KD>();
+            }
+            if (late) await(j0 + 2 < j1);
+            barrier();
+            for (int j = j0; j < jw - 1; ++j) {
+                begin_w(j);
+                weigh(j);
+                end_w(j);
+                collect(j);
+                scores(j + 1);
+                order_turn<4 * ND, 2 * KD>();
+                end_m(j);
+            }
+            if (j0 < jw) {
+                begin_w(jw - 1);
+                weigh(jw - 1);
+                end_w(jw - 1);
+                collect(jw - 1);
+                order_turn<4 * ND, 0>();
+                end_m(jw - 1);
+            }
+            for (int j = jw; j < j1; ++j) {
+                begin_w(j);
+                end_w(j);
+                end_m(j);
+            }
+            if (!late) barrier();
+        }
+    } else {
+        for (int j = j0; j < j1; ++j) {
+            wait_vm<0>();
+            barrier();  // every wave's part of tile j is there, and nobody reads the other stage any more
+            if (j + 1 < j1) {
+                issue(j + 1);
+                find_pages(j + 2);
+            }
+            if (unsafe(j)) {
+                make_safe(j, threadIdx.x, 64 * NW);
+                barrier();
+            }
+            if (active && lim_hi >= j * kTile) {
+                scores(j);
+                weigh(j);
+                collect(j);
             }
         }
-#pragma unroll
-        for (int d = 0; d < ND; ++d)
-#pragma unroll
-            for (int ks = 0; ks < 4; ++ks) o[d] = mfma32<F16>(v_operand(d, ks), pb[ks], o[d]);
     }
 
     if (bad) bad_l = 1;  // any wave's
     barrier();
     if (!active) return;
+    if (odd_l) {
+#pragma unroll 1
+        for (int p = max(j0 * kTile, (lim_wg + 1) & ~(kTile - 1)); p < min(j1 * kTile, t.end); ++p) {
+            const uint8_t* vr = vbase + page_offset(a.kv, trow, a.width, p, bad) + 8 * hf;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint2 u = *reinterpret_cast<const uint2*>(vr + 64 * d + 16 * e);
+                    if (p <= lim && (nonfinite2<F16>(u.x) || nonfinite2<F16>(u.y))) {
+                        o[d][4 * e] += lo_of<F16>(u.x) - lo_of<F16>(finite2<F16>(u.x));
+                        o[d][4 * e + 1] += hi_of<F16>(u.x) - hi_of<F16>(finite2<F16>(u.x));
+                        o[d][4 * e + 2] += lo_of<F16>(u.y) - lo_of<F16>(finite2<F16>(u.y));
+                        o[d][4 * e + 3] += hi_of<F16>(u.y) - hi_of<F16>(finite2<F16>(u.y));
+                    }
+                }
+        }
+    }
     l = add_xor32(l);
     const bool poison = bad_l != 0;
     if (row >= t.rows) return;
@@ -490,7 +612,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_flat(const FlatA
     }
     if (b < 0) return;
     bool bad = false;
-    len = held(a.kv_len[b], a.width, a.kv.shift, bad);
+    len = held(scalar_at(a.kv_len, b), a.width, a.kv.shift, bad);
     if (piece == 0 && hr == 0 && threadIdx.x == 0) {
         a.first[2 * b] = before;
         a.first[2 * b + 1] = pieces;
@@ -502,14 +624,36 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_flat(const FlatA
     const uint8_t* vbase = a.kv.vc + head * a.kv.hs;
     uint8_t *ks = &slot[wv][0][0], *vs = &slot[wv][1][0];
     const int dr = lane / (RB / 16), dc = lane % (RB / 16);
-    const int last_row = (to - 1) & ~(RPI - 1);
+    // The page ids of the 32 positions from p on (16 are always in one page; rows past the end repeat the last 16: their
+    // page exists), read an iteration before its loads are issued.
+    int page[2];
+    auto half_at = [&](int p, int h) { return min(p + 16 * h, (to - 1) & ~15); };
+    auto find_pages = [&](int p) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int at = half_at(p, h) >> a.kv.shift;
+            page[h] = scalar_at(trow, min(at, a.width - 1));
+            if (at >= a.width) page[h] = -1;
+        }
+    };
+    // the lane's offset in an instruction's rows: the permutations have period 16 in the row
+    constexpr int SAME = 16 / RPI;
+    uint32_t ko[SAME], vo[SAME];
+#pragma unroll
+    for (int i = 0; i < SAME; ++i) {
+        const int rr = RPI * i + dr;
+        ko[i] = (uint32_t)((rr & 15) * (int)a.kv.rs + 16 * swz_k<D>(rr, dc));
+        vo[i] = (uint32_t)((rr & 15) * (int)a.kv.rs + 16 * swz_v<D, true>(rr, dc));
+    }
     auto issue = [&](int p, bool v) {
 #pragma unroll
-        for (int i = 0; i < LI; ++i) {
-            const int rr = RPI * i + dr;
-            const int64_t off = page_offset(a.kv, trow, a.width, min(p + RPI * i, last_row), bad);
-            const uint32_t lo = (uint32_t)(dr * (int)a.kv.rs + 16 * (v ? swz_v<D, true>(rr, dc) : swz_k<D>(rr, dc)));
-            dma16(lds_addr((v ? vs : ks) + 1024 * i), uniform((v ? vbase : kbase) + off), lo);
+        for (int h = 0; h < 2; ++h) {
+            const bool ok = (unsigned)page[h] < (unsigned)a.kv.pages;
+            bad = bad || !ok;
+            const int64_t off = (ok ? (int64_t)page[h] : 0) * a.kv.ps + (int64_t)(half_at(p, h) & ((1 << a.kv.shift) - 1)) * a.kv.rs;
+            const uint8_t* base = uniform((v ? vbase : kbase) + off);
+#pragma unroll
+            for (int i = 0; i < LI / 2; ++i) dma16(lds_addr((v ? vs : ks) + 1024 * (h * (LI / 2) + i)), base, v ? vo[i] : ko[i]);
         }
     };
     const int p_first = from + kSub * wv;
@@ -523,8 +667,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_flat(const FlatA
 #pragma unroll
     for (int k = 0; k < KD; ++k) asm volatile("" : "+v"(qb[k].x), "+v"(qb[k].y), "+v"(qb[k].z), "+v"(qb[k].w));
     if (p_first < to) {
+        find_pages(p_first);
         issue(p_first, false);
         issue(p_first, true);
+        find_pages(p_first + kStep);
     }
 
     f4_t o[ND];
@@ -603,7 +749,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_flat(const FlatA
             va[d] = make_uint4(x.x, x.y, y.x, y.y);
         }
         wait_lds();  // the V slot is read
-        if (more) issue(p + kStep, true);
+        if (more) {
+            issue(p + kStep, true);
+            find_pages(p + 2 * kStep);
+        }
 #pragma unroll
         for (int d = 0; d < ND; ++d) o[d] = mfma16<F16>(va[d], make_uint4(hi[0], hi[1], hi[2], hi[3]), o[d]);
 #pragma unroll
