@@ -463,9 +463,11 @@ __global__ __launch_bounds__(64 * NW, 1) void k_attn_rows(const RowsArgs a, int 
                 begin_w(j);
                 weigh(j);
                 end_w(j);
+                __builtin_amdgcn_s_setprio(1);
                 collect(j);
                 scores(j + 1);
                 order_turn<4 * ND, 2 * KD>();
+                __builtin_amdgcn_s_setprio(0);
                 end_m(j);
             }
             if (j0 < jw) {
