@@ -154,6 +154,11 @@ def stream(device: torch.device) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+def raw_stream(device: torch.device) -> int:
+    """The current stream's handle, as stream() gives it, without the Stream object (2 us of a small call)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
 def require_gpu(*tensors: torch.Tensor, what: str) -> torch.device:
     dev = None
     for t in tensors:

@@ -539,6 +539,8 @@ def dl_route(logits, k, norm_topk, row, host_row=None, host_flag=None, seq=None)
 
 
 # ----------------------------------------------------------------------------- a paged K/V cache of several sequences
+# (These wrappers are the better part of a small call's time: they read each tensor's properties once, pass plain integers
+# and take the raw stream handle.)
 _CACHE_DTYPES = {torch.bfloat16: _lib.WISP_DT_BF16, torch.float16: _lib.WISP_DT_F16}
 
 
@@ -548,36 +550,55 @@ def _int32(t, n, what):
     assert t.numel() == n, f"{what} must have {n} elements (got {t.numel()})"
 
 
-def _paged_cache(q, kc, vc, table, hq, what):
-    """Checks of a paged cache and its tables against q [.., hq, D]; the C entry points' cache arguments."""
-    D = q.shape[-1]
-    dt = _CACHE_DTYPES.get(q.dtype)
-    if dt is None or kc.dtype != q.dtype or vc.dtype != q.dtype:
-        raise TypeError(f"{what} takes bfloat16 or float16 of one dtype (got {q.dtype}, {kc.dtype}, {vc.dtype})")
-    assert kc.dim() == 4 and kc.shape == vc.shape and kc.shape[3] == D, "caches must be [pages, Hk, page, D]"
-    assert kc.stride(3) == 1 and kc.stride() == vc.stride(), "caches need contiguous rows and equal strides"
-    assert hq % kc.shape[1] == 0, f"{hq} query heads over {kc.shape[1]} K/V heads"
+def _paged_cache(q, kc, vc, table, what):
+    """Checks of a paged cache and its tables against q [.., hq, D]: (WISP_DT_* code, B, table width, K/V heads, the C entry
+    points' cache arguments)."""
+    _, hq, D = q.shape
+    dtype = q.dtype
+    dt = _CACHE_DTYPES.get(dtype)
+    if dt is None or kc.dtype != dtype or vc.dtype != dtype:
+        raise TypeError(f"{what} takes bfloat16 or float16 of one dtype (got {dtype}, {kc.dtype}, {vc.dtype})")
+    shape, st = kc.shape, kc.stride()
+    assert len(shape) == 4 and shape == vc.shape and shape[3] == D, "caches must be [pages, Hk, page, D]"
+    assert st[3] == 1 and st == vc.stride(), "caches need contiguous rows and equal strides"
+    P, hk, page, _ = shape
+    assert hq % hk == 0, f"{hq} query heads over {hk} K/V heads"
     if table.dtype != torch.int32 or table.dim() != 2 or not table.is_contiguous():
         raise TypeError("table must be a contiguous int32 [B, pages of a sequence] tensor")
-    cache = (_lib.ptr(kc), _lib.ptr(vc), kc.shape[0], kc.shape[2], kc.stride(0), kc.stride(1), kc.stride(2))
-    return dt, cache
+    B, width = table.shape
+    return dt, B, width, hk, (kc.data_ptr(), vc.data_ptr(), P, page, st[0], st[1], st[2])
 
 
 def _rows(x, what):
-    """x [T, h, D] with contiguous D: x, or a copy where its strides or address are not ones that the kernels read."""
-    assert x.dim() == 3, f"{what} must be [tokens, heads, D]"
-    if x.stride(2) != 1 or x.stride(0) % 8 or x.stride(1) % 8 or x.data_ptr() % 16:
+    """x [T, h, D] with contiguous D and its token and head strides: x, or a copy where its strides or address are not ones
+    that the kernels read."""
+    st = x.stride()
+    assert len(st) == 3, f"{what} must be [tokens, heads, D]"
+    if st[2] != 1 or st[0] % 8 or st[1] % 8 or x.data_ptr() % 16:
         x = x.contiguous()
         if x.data_ptr() % 16:
             x = x.clone()
-    return x
+        st = x.stride()
+    return x, x.data_ptr(), st[0], st[1]
 
 
 def _out(out, shape, like):
     if out is None:
         return torch.empty(shape, dtype=like.dtype, device=like.device)
     assert out.shape == shape and out.dtype == like.dtype and out.is_contiguous(), f"out must be a contiguous {shape} tensor"
+    assert out.device == like.device
     return out
+
+
+def _call(dev, fn, args, what):
+    """fn(*args, the current stream of dev) with dev as the current device."""
+    if torch.cuda.current_device() == dev.index:
+        rc = fn(*args, _lib.raw_stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _lib.raw_stream(dev))
+    if rc:
+        _lib.check(rc, what)
 
 
 def kv_append(q, k, v, cos, sin, cu, kv_len, table, kc, vc, q_norm_w=None, k_norm_w=None, eps=1e-6, interleaved=False,
@@ -593,31 +614,30 @@ def kv_append(q, k, v, cos, sin, cu, kv_len, table, kc, vc, q_norm_w=None, k_nor
     pairs (i, i + R/2), or (2i, 2i + 1) where interleaved. float32 throughout, rounded once.
     Returns the rotated q [T, Hq, D]; its rows from cu[B] on are left as they were (qo) or undefined."""
     T, hq, D = q.shape
-    hk, B = kc.shape[1], table.shape[0]
-    dt, cache = _paged_cache(q, kc, vc, table, hq, "kv_append")
-    norms = [w for w in (q_norm_w, k_norm_w) if w is not None]
+    dt, B, width, hk, cache = _paged_cache(q, kc, vc, table, "kv_append")
+    dtype = q.dtype
+    assert (q_norm_w is None) == (k_norm_w is None), "q_norm_w and k_norm_w: both or neither"
+    norms = () if q_norm_w is None else (q_norm_w, k_norm_w)
     dev = _lib.require_gpu(q, k, v, cos, sin, cu, kv_len, table, kc, vc, *norms, what="kv_append")
-    assert k.shape == (T, hk, D) and v.shape == (T, hk, D) and k.dtype == v.dtype == q.dtype
+    assert k.shape == (T, hk, D) and v.shape == (T, hk, D) and k.dtype == dtype and v.dtype == dtype
     _int32(cu, B + 1, "cu")
     _int32(kv_len, B, "kv_len")
     assert cos.dim() == 2 and cos.shape == sin.shape and cos.dtype == sin.dtype, "cos and sin must be [positions, R]"
-    if cos.dtype not in (q.dtype, torch.float32):
-        raise TypeError(f"cos and sin must be float32 or {q.dtype} (got {cos.dtype})")
-    assert len(norms) != 1, "q_norm_w and k_norm_w: both or neither"
+    if cos.dtype != dtype and cos.dtype != torch.float32:
+        raise TypeError(f"cos and sin must be float32 or {dtype} (got {cos.dtype})")
     for w in norms:
-        assert w.dtype == q.dtype and w.shape == (D,) and w.is_contiguous(), "norm weights must be [D] of q's dtype"
-    q, k, v, cos, sin = _rows(q, "q"), _rows(k, "k"), _rows(v, "v"), cos.contiguous(), sin.contiguous()
+        assert w.dtype == dtype and w.shape == (D,) and w.is_contiguous(), "norm weights must be [D] of q's dtype"
+    q, qp, q_ts, q_hs = _rows(q, "q")
+    k, kp, k_ts, k_hs = _rows(k, "k")
+    v, vp, v_ts, v_hs = _rows(v, "v")
+    cos, sin = cos.contiguous(), sin.contiguous()
     qo = _out(qo, (T, hq, D), q)
-    with torch.cuda.device(dev):
-        _lib.check(
-            _lib.lib().wisp_kv_append(
-                _lib.ptr(q), q.stride(0), q.stride(1), _lib.ptr(k), k.stride(0), k.stride(1), _lib.ptr(v), v.stride(0),
-                v.stride(1), _lib.ptr(q_norm_w), _lib.ptr(k_norm_w), float(eps), _lib.ptr(cos), _lib.ptr(sin),
-                cos.shape[0], cos.shape[1], _X_DTYPES[cos.dtype], int(bool(interleaved)), _lib.ptr(cu), _lib.ptr(kv_len),
-                _lib.ptr(table), table.shape[1], B, T, hq, hk, D, dt, *cache, _lib.ptr(qo), _lib.stream(dev),
-            ),
-            "kv_append",
-        )
+    qw, kw = (w.data_ptr() for w in norms) if norms else (None, None)
+    rows, rot = cos.shape
+    _call(dev, _lib.lib().wisp_kv_append,
+          (qp, q_ts, q_hs, kp, k_ts, k_hs, vp, v_ts, v_hs, qw, kw, eps, cos.data_ptr(), sin.data_ptr(), rows, rot,
+           _X_DTYPES[cos.dtype], 1 if interleaved else 0, cu.data_ptr(), kv_len.data_ptr(), table.data_ptr(), width, B, T,
+           hq, hk, D, dt, *cache, qo.data_ptr()), "kv_append")
     return qo
 
 
@@ -628,55 +648,43 @@ def attn_prompt(q, kc, vc, cu, kv_len, table, scale, out=None):
     were (out) or undefined. Nothing is read back to the host, so the call can be captured and the lengths changed between
     replays."""
     T, hq, D = q.shape
-    hk, B = kc.shape[1], table.shape[0]
-    dt, cache = _paged_cache(q, kc, vc, table, hq, "attn_prompt")
+    dt, B, width, hk, cache = _paged_cache(q, kc, vc, table, "attn_prompt")
     dev = _lib.require_gpu(q, kc, vc, cu, kv_len, table, what="attn_prompt")
     _int32(cu, B + 1, "cu")
     _int32(kv_len, B, "kv_len")
-    q = _rows(q, "q")
+    q, qp, q_ts, q_hs = _rows(q, "q")
     out = _out(out, (T, hq, D), q)
     L = _lib.lib()
-    nb = L.wisp_attn_prompt_ws_bytes(T, B, hq, hk, D, kc.shape[2], table.shape[1])
-    with torch.cuda.device(dev):
-        ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb > 0 else None
-        _lib.check(
-            L.wisp_attn_prompt(
-                _lib.ptr(q), q.stride(0), q.stride(1), *cache, _lib.ptr(cu), _lib.ptr(kv_len), _lib.ptr(table),
-                table.shape[1], B, T, hq, hk, D, dt, float(scale), _lib.ptr(ws), _lib.ptr(out), _lib.stream(dev),
-            ),
-            "attn_prompt",
-        )
+    nb = L.wisp_attn_prompt_ws_bytes(T, B, hq, hk, D, cache[3], width)
+    ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb > 0 else None
+    _call(dev, L.wisp_attn_prompt,
+          (qp, q_ts, q_hs, *cache, cu.data_ptr(), kv_len.data_ptr(), table.data_ptr(), width, B, T, hq, hk, D, dt, scale,
+           None if ws is None else ws.data_ptr(), out.data_ptr()), "attn_prompt")
     return out
 
 
-def _attn_batch(q, kc, vc, kv_len, table, prefix_len, prefix_table, scale, out, what):
-    B, hq, D = q.shape
-    hk = kc.shape[1]
-    dt, cache = _paged_cache(q, kc, vc, table, hq, what)
-    assert table.shape[0] == B, f"{B} rows of q, {table.shape[0]} of table"
-    pre = [t for t in (prefix_len, prefix_table) if t is not None]
-    dev = _lib.require_gpu(q, kc, vc, kv_len, table, *pre, what=what)
+def _attn_batch(q, kc, vc, kv_len, table, prefix, scale, out, what):
+    n, hq, D = q.shape
+    dt, B, width, hk, cache = _paged_cache(q, kc, vc, table, what)
+    assert B == n, f"{n} rows of q, {B} of table"
+    dev = _lib.require_gpu(q, kc, vc, kv_len, table, *prefix, what=what)
     _int32(kv_len, B, "kv_len")
-    width = 0
-    if pre:
-        width = prefix_table.numel()
-        _int32(prefix_len, 1, "prefix_len")
-        _int32(prefix_table, width, "prefix_table")
-        assert prefix_table.dim() == 1 and width >= 1, "prefix_table must be [pages of the prefix]"
-    q = _rows(q, "q")
+    pre = (None, None, 0)
+    if prefix:
+        plen, ptable = prefix
+        pw = ptable.numel()
+        _int32(plen, 1, "prefix_len")
+        _int32(ptable, pw, "prefix_table")
+        assert ptable.dim() == 1 and pw >= 1, "prefix_table must be [pages of the prefix]"
+        pre = (plen.data_ptr(), ptable.data_ptr(), pw)
+    q, qp, q_ts, q_hs = _rows(q, "q")
     out = _out(out, (B, hq, D), q)
     L = _lib.lib()
-    nb = L.wisp_attn_batch_ws_bytes(B, hq, hk, D, kc.shape[2], width)
-    with torch.cuda.device(dev):
-        ws = torch.empty(max(nb, 0), dtype=torch.uint8, device=dev)
-        _lib.check(
-            L.wisp_attn_batch(
-                _lib.ptr(q), q.stride(0), q.stride(1), *cache, _lib.ptr(kv_len), _lib.ptr(table), table.shape[1],
-                _lib.ptr(prefix_len), _lib.ptr(prefix_table), width, B, hq, hk, D, dt, float(scale), _lib.ptr(ws),
-                _lib.ptr(out), _lib.stream(dev),
-            ),
-            what,
-        )
+    nb = L.wisp_attn_batch_ws_bytes(B, hq, hk, D, cache[3], pre[2])
+    ws = torch.empty(max(nb, 0), dtype=torch.uint8, device=dev)
+    _call(dev, L.wisp_attn_batch,
+          (qp, q_ts, q_hs, *cache, kv_len.data_ptr(), table.data_ptr(), width, *pre, B, hq, hk, D, dt, scale, ws.data_ptr(),
+           out.data_ptr()), what)
     return out
 
 
@@ -684,11 +692,11 @@ def attn_batch(q, kc, vc, kv_len, table, scale, out=None):
     """attn_decode for a batch: one token of each of B sequences, q [B, Hq, D] (bf16 or f16), over the kv_len[b] positions
     that sequence b has in the paged cache kc, vc [pages, Hk, page, D] (kv_len int32 [B] and table int32 [B, pages of a
     sequence] on the GPU; a sequence without positions gives zeros). Returns [B, Hq, D]."""
-    return _attn_batch(q, kc, vc, kv_len, table, None, None, scale, out, "attn_batch")
+    return _attn_batch(q, kc, vc, kv_len, table, (), scale, out, "attn_batch")
 
 
 def attn_shared(q, kc, vc, kv_len, table, prefix_len, prefix_table, scale, out=None):
     """attn_batch for sequences that begin with the same prefix: every row of q first attends the prefix_len[0] (int32 [1])
     positions in the pages prefix_table (int32 [pages of the prefix]), whose keys and values are read once for the whole
     batch, then its own kv_len[b] positions in table[b]."""
-    return _attn_batch(q, kc, vc, kv_len, table, prefix_len, prefix_table, scale, out, "attn_shared")
+    return _attn_batch(q, kc, vc, kv_len, table, (prefix_len, prefix_table), scale, out, "attn_shared")
