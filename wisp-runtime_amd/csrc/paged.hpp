@@ -42,14 +42,24 @@ __device__ __forceinline__ int held(int len, int width, int shift, bool& bad) {
     return min(max(len, 0), cap);
 }
 
-// Inclusive sum of v over the lanes up to this one.
-__device__ __forceinline__ int wave_scan(int v, int lane) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int u = __shfl_up(v, o, 64);
-        if (lane >= o) v += u;
-    }
+// Inclusive sum of v over the lanes up to this one: four DPP shifts in each row of 16, then the row totals handed on.
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr:1
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);  // row_shr:2
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);  // row_shr:4
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);  // row_shr:8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast:15 into rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast:31 into rows 2 and 3
     return v;
+}
+
+// x / d for x >= 0, d >= 1 and a quotient below 2^20: that of floats is off by one at most.
+__device__ __forceinline__ int small_div(int x, int d) {
+    int q = (int)((float)x * __builtin_amdgcn_rcpf((float)d));
+    const int r = x - q * d;
+    if (r < 0) --q;
+    if (r >= d) ++q;
+    return q;
 }
 
 // Sequence b's tokens in a pack: rows [lo, hi) of cu, kept inside [0, T] whatever cu holds.

@@ -42,6 +42,7 @@ constexpr int kTile = 64;          // positions per tile of k_attn_rows
 constexpr int kSub = 32;           // positions per slot of k_attn_flat
 constexpr int kStep = 4 * kSub;    // positions of a workgroup's four slots: the grain of its pieces
 constexpr float kLazy = 6.f;       // m follows the maximum past 2^kLazy
+constexpr int kSlotsY = 32768;     // grid.y of k_attn_rows
 constexpr int kPieces = 1024;      // pieces that k_attn_flat aims at over all sequences and K/V heads
 
 // float16 weights p: times 2^8, so that small ones keep their bits (the grain 2^-24 is then 2^-32 of the largest) and
@@ -127,17 +128,17 @@ __device__ __forceinline__ int swz_v(int r, int c) {
     return c ^ (D == 64 ? ((r >> 1) & 1) << 2 : (r & 3) << 2);
 }
 
-// A non-finite value in a pair: exponent bits all set.
+// Where a pair holds a non-finite value (exponent bits all set): the sign bits of its halves.
 template <bool F16>
-__device__ __forceinline__ bool nonfinite2(uint32_t u) {
-    constexpr uint32_t M = F16 ? 0x7C00u : 0x7F80u;
-    return (u & M) == M || ((u >> 16) & M) == M;
+__device__ __forceinline__ uint32_t nonfinite2(uint32_t u) {
+    constexpr uint32_t M = F16 ? 0x7C007C00u : 0x7F807F80u, ONE = F16 ? 0x04000400u : 0x00800080u;
+    return ((u & M) + ONE) & 0x80008000u;
 }
 // The values of a pair that are finite, others as 0.
 template <bool F16>
 __device__ __forceinline__ uint32_t finite2(uint32_t u) {
-    constexpr uint32_t M = F16 ? 0x7C00u : 0x7F80u;
-    return ((u & M) == M ? 0u : u & 0xFFFFu) | (((u >> 16) & M) == M ? 0u : u & 0xFFFF0000u);
+    const uint32_t n = nonfinite2<F16>(u);
+    return (n & 0x8000u ? 0u : u & 0xFFFFu) | (n >> 31 ? 0u : u & 0xFFFF0000u);
 }
 
 // The order of a turn's LDS reads and matrix instructions: NV operands of V (two reads each), then NK of K (one read), each
@@ -158,8 +159,9 @@ struct RowsArgs {
     int64_t q_ts, q_hs;  // elements
     PagedKV kv;
     const int *cu, *kv_len, *table;  // cu null: one sequence of B rows, none of which is masked (a shared prefix)
-    int width, B, T, hq, hk;
-    float c;        // scale * log2(e)
+    int width, B, T, hq, hk, G;
+    float per_group;  // 1 / G
+    float c;          // scale * log2(e)
     int nsplit;     // parts that the grid has for each row tile
     int part_min;   // tiles that a part is worth
     float *ml, *po;  // records of split row tiles: [(token * hq + head) * nsplit + part][2] and [..][D]
@@ -167,56 +169,68 @@ struct RowsArgs {
 };
 
 struct RowTile {
-    int b, tok0, rows, r0, off, end;  // sequence, its first token, its rows, the tile's first row, position of token 0,
-                                      // positions that the tile's rows attend
-    bool bad;                         // the sequence is longer than its table
+    int b, rows, off, end;      // sequence, its rows, position of its token 0, positions that the tile's rows attend
+    int first, tok0, rem, left; // q row of the sequence's token 0; the tile's first row is head rem of the group of token
+                                // tok0, and left rows of the sequence begin with it
+    bool bad;                   // the sequence is longer than its table
 };
 // Parts that a row tile's positions are cut into: no more than nsplit, and part_min tiles each.
 __device__ __forceinline__ int parts_of(int tiles, int nsplit, int part_min) {
     return max(1, min(nsplit, tiles / part_min));
 }
-__device__ __forceinline__ int tile_end(int off, int rows, int r0, int bm, int G, int len) {
-    const int last = off + (min(r0 + bm, rows) - 1) / G;
-    return max(0, min(len, last + 1));
+// Of a tile whose rows are those from head rem of token tok0 on: token of its row x (x + rem < 2^11).
+__device__ __forceinline__ int token_of(int tok0, int rem, int x, float per_group) {
+    return tok0 + (int)(((float)(rem + x) + 0.5f) * per_group);
 }
 
 // Row tile number s of the pack (tiles of BM rows, sequence after sequence), or false.
 template <int BM>
 __device__ __forceinline__ bool find_tile(const RowsArgs& a, int s, int lane, RowTile& t) {
-    const int G = a.hq / a.hk;
+    const int G = a.G;
     t.bad = false;
+    if (s < 0) return false;
+    int r0;
     if (!a.cu) {
-        t.b = 0, t.tok0 = 0, t.rows = a.B * G, t.r0 = s * BM;
-        t.off = 0;
-        t.end = held(scalar_at(a.kv_len, 0), a.width, a.kv.shift, t.bad);
-        return t.r0 < t.rows;
-    }
-    int before = 0;
-    for (int b0 = 0; b0 < a.B; b0 += 64) {
-        int lo = 0, hi = 0;
-        if (b0 + lane < a.B) token_range(a.cu, b0 + lane, a.T, lo, hi);
-        const int n = ((hi - lo) * G + BM - 1) / BM;
-        const int sum = before + wave_scan(n, lane);
-        const uint64_t mine = __ballot(s < sum);
-        if (mine) {
-            const int w = __builtin_ctzll(mine);
-            t.b = b0 + w;
-            t.tok0 = __builtin_amdgcn_readlane(lo, w);
-            const int n_tok = __builtin_amdgcn_readlane(hi, w) - t.tok0;
-            t.rows = n_tok * G;
-            t.r0 = (s - (__builtin_amdgcn_readlane(sum, w) - __builtin_amdgcn_readlane(n, w))) * BM;
-            const int len = held(scalar_at(a.kv_len, t.b), a.width, a.kv.shift, t.bad);
-            t.off = len - n_tok;
-            t.end = tile_end(t.off, t.rows, t.r0, BM, G, len);
-            return true;
+        t.b = 0, t.first = 0, t.rows = a.B * G, r0 = s * BM;
+        if (r0 >= t.rows) return false;
+    } else {
+        int before = 0;
+        bool found = false;
+        for (int b0 = 0; b0 < a.B && !found; b0 += 64) {
+            int lo = 0, hi = 0;
+            if (b0 + lane < a.B) token_range(a.cu, b0 + lane, a.T, lo, hi);
+            const int n = ((hi - lo) * G + BM - 1) / BM;
+            const int sum = before + wave_scan(n);
+            const uint64_t mine = __ballot(s < sum);
+            if (mine) {
+                const int w = __builtin_ctzll(mine);
+                t.b = b0 + w;
+                t.first = __builtin_amdgcn_readlane(lo, w);
+                t.rows = (__builtin_amdgcn_readlane(hi, w) - t.first) * G;
+                r0 = (s - (__builtin_amdgcn_readlane(sum, w) - __builtin_amdgcn_readlane(n, w))) * BM;
+                found = true;
+            } else {
+                before = __builtin_amdgcn_readlane(sum, 63);
+            }
         }
-        before = __builtin_amdgcn_readlane(sum, 63);
+        if (!found) return false;
     }
-    return false;
+    const int len = held(scalar_at(a.kv_len, t.b), a.width, a.kv.shift, t.bad);
+    t.tok0 = (int)((uint32_t)r0 / (uint32_t)G);
+    t.rem = r0 - t.tok0 * G;
+    t.left = t.rows - r0;
+    t.off = 0;
+    t.end = len;
+    if (a.cu) {
+        t.off = len - (int)((uint32_t)t.rows / (uint32_t)G);
+        const int last = __builtin_amdgcn_readfirstlane(token_of(t.tok0, t.rem, min(BM, t.left) - 1, a.per_group));
+        t.end = max(0, t.off + last + 1);
+    }
+    return true;
 }
 
-// Grid: blockIdx.x = (slot * nsplit + part) * hk + head, so that a head's workgroups mostly share an XCD's L2 (hk a
-// divisor or multiple of 8); slots count down, since a prompt's last rows have the most positions.
+// Grid: x = part * hk + head, so that a head's workgroups mostly share an XCD's L2 (hk a divisor or multiple of 8); y and z:
+// the slot, counting down, since a prompt's last rows have the most positions.
 //
 // A tile costs a wave 4 D / 8 matrix instructions of 32 cycles each (S and O, 1,024 cycles at D = 128) and about as many
 // VALU cycles (32 weights per lane), and the LDS reads of its operands are as long. With eight waves, two to a SIMD, the
@@ -236,15 +250,16 @@ __global__ __launch_bounds__(64 * NW, 1) void k_attn_rows(const RowsArgs a, int 
     __shared__ int bad_l, odd_l;  // a page that does not exist; an infinite or NaN value taken out of V
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 31, hf = lane >> 5;
-    const int G = a.hq / a.hk;
-    const int head = blockIdx.x % a.hk, rest = blockIdx.x / a.hk;
-    const int part = rest % a.nsplit, slot = slots - 1 - rest / a.nsplit;
+    const int G = a.G;
+    const int part = a.nsplit > 1 ? blockIdx.x / a.hk : 0, head = blockIdx.x - part * a.hk;
+    const int slot = slots - 1 - (int)(blockIdx.y + kSlotsY * blockIdx.z);
     RowTile t;
     if (!find_tile<BM>(a, slot, lane, t)) return;
     const int tiles = (t.end + kTile - 1) / kTile;
     const int parts = a.out ? parts_of(tiles, a.nsplit, a.part_min) : a.nsplit;
     if (part >= parts) return;
-    const int j0 = (int)((int64_t)tiles * part / parts), j1 = (int)((int64_t)tiles * (part + 1) / parts);
+    // (tiles <= 2^24, parts <= 256)
+    const int j0 = parts > 1 ? (uint32_t)tiles * part / parts : 0, j1 = parts > 1 ? (uint32_t)tiles * (part + 1) / parts : tiles;
     if (threadIdx.x == 0) bad_l = odd_l = 0;
 
     const int* trow = a.table + (int64_t)t.b * a.width;
@@ -295,16 +310,16 @@ __global__ __launch_bounds__(64 * NW, 1) void k_attn_rows(const RowsArgs a, int 
     find_pages(j0 + lead);
 
     // this lane's query row: (token, head of the group); rows past the sequence's repeat its last and are not stored
-    const int row = t.r0 + 32 * wv + n, rr = min(row, t.rows - 1);
-    const int tok = rr / G, g = rr - tok * G;
-    const int lim = a.cu ? min(t.off + tok, t.end - 1) : t.end - 1;
-    const int wrow = t.r0 + 32 * wv;
-    const bool active = wrow < t.rows;
-    const int lim_lo = a.cu ? t.off + min(wrow, t.rows - 1) / G : t.end - 1;       // the wave's first row's
-    const int lim_hi = a.cu ? t.off + min(wrow + 31, t.rows - 1) / G : t.end - 1;  // and last row's
+    const int x = 32 * wv + n, xx = min(x, t.left - 1);
+    const int tok = token_of(t.tok0, t.rem, xx, a.per_group), g = t.rem + xx - (tok - t.tok0) * G;
+    const int lim = a.cu ? t.off + tok : t.end - 1;
+    const bool active = 32 * wv < t.left;
+    // limits of the workgroup's first row, and of the wave's first and last
+    const int lim_wg = a.cu ? t.off + t.tok0 : t.end - 1;
+    const int lim_lo = __builtin_amdgcn_readfirstlane(lim), lim_hi = __builtin_amdgcn_readlane(lim, 31);
     uint4 qb[KD];
     {
-        const uint16_t* qr = a.q + (int64_t)(t.tok0 + tok) * a.q_ts + (int64_t)(head * G + g) * a.q_hs + 8 * hf;
+        const uint16_t* qr = a.q + (int64_t)(t.first + tok) * a.q_ts + (int64_t)(head * G + g) * a.q_hs + 8 * hf;
 #pragma unroll
         for (int s = 0; s < KD; ++s) qb[s] = *reinterpret_cast<const uint4*>(qr + 16 * s);
     }
@@ -353,7 +368,7 @@ __global__ __launch_bounds__(64 * NW, 1) void k_attn_rows(const RowsArgs a, int 
             for (int u = 0; u < 2; ++u)
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    if (p0 + 32 * u + 8 * (i >> 2) + 4 * hf + (i & 3) > lim) s[u][i] = -INFINITY;
+                    if (32 * u + 8 * (i >> 2) + (i & 3) > lim - p0 - 4 * hf) s[u][i] = -INFINITY;
         }
         float mx = s[0][0];
 #pragma unroll
@@ -404,14 +419,13 @@ __global__ __launch_bounds__(64 * NW, 1) void k_attn_rows(const RowsArgs a, int 
     // Where a tile has positions that not all rows attend, V must hold nothing that weight 0 would not erase: rows past the
     // end, which may hold anything, are cleared, and an infinite or NaN value is taken out and added at the end to those
     // rows that attend it. By the threads first, first + many, ..
-    const int lim_wg = a.cu ? t.off + t.r0 / G : t.end - 1;  // the tile's first row's limit
     auto unsafe = [&](int j) { return (j + 1) * kTile - 1 > lim_wg; };
     auto make_safe = [&](int j, int first, int many) {
         uint8_t* vt = &buf[j & (NST - 1)][1][0];
         const int tail = (t.end - j * kTile) * (RB / 16);
         for (int e = first; e < kTile * (RB / 16); e += many) {
             uint4 u = e < tail ? *reinterpret_cast<const uint4*>(vt + 16 * e) : make_uint4(0, 0, 0, 0);
-            const bool odd = nonfinite2<F16>(u.x) || nonfinite2<F16>(u.y) || nonfinite2<F16>(u.z) || nonfinite2<F16>(u.w);
+            const bool odd = nonfinite2<F16>(u.x) | nonfinite2<F16>(u.y) | nonfinite2<F16>(u.z) | nonfinite2<F16>(u.w);
             if (odd) {
                 u = make_uint4(finite2<F16>(u.x), finite2<F16>(u.y), finite2<F16>(u.z), finite2<F16>(u.w));
                 odd_l = 1;
@@ -517,7 +531,7 @@ __global__ __launch_bounds__(64 * NW, 1) void k_attn_rows(const RowsArgs a, int 
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const uint2 u = *reinterpret_cast<const uint2*>(vr + 64 * d + 16 * e);
-                    if (p <= lim && (nonfinite2<F16>(u.x) || nonfinite2<F16>(u.y))) {
+                    if (p <= lim && (nonfinite2<F16>(u.x) | nonfinite2<F16>(u.y))) {
                         o[d][4 * e] += lo_of<F16>(u.x) - lo_of<F16>(finite2<F16>(u.x));
                         o[d][4 * e + 1] += hi_of<F16>(u.x) - hi_of<F16>(finite2<F16>(u.x));
                         o[d][4 * e + 2] += lo_of<F16>(u.y) - lo_of<F16>(finite2<F16>(u.y));
@@ -528,8 +542,8 @@ __global__ __launch_bounds__(64 * NW, 1) void k_attn_rows(const RowsArgs a, int 
     }
     l = add_xor32(l);
     const bool poison = bad_l != 0;
-    if (row >= t.rows) return;
-    const int64_t orow = (int64_t)(t.tok0 + tok) * a.hq + head * G + g;
+    if (x >= t.left) return;
+    const int64_t orow = (int64_t)(t.first + tok) * a.hq + head * G + g;
     if (a.out && parts == 1) {
         const float inv = poison ? __int_as_float(0x7FC00000) : l == 0.f ? 0.f : 1.f / l;
         uint16_t* dst = a.out + orow * D + 4 * hf;
@@ -561,24 +575,17 @@ struct FlatArgs {
     int64_t q_ts, q_hs;
     PagedKV kv;
     const int *kv_len, *table;
-    int width, B, hq, hk;
+    int width, B, hq, hk, G, want;
     float c;
     int* first;      // [B][2]: number of the sequence's first piece, its pieces
     float *ml, *po;  // records [(first + piece) * hq + head]
     uint16_t* out;   // [B][hq][D]; null: every piece leaves a record (a prefix's are to be added)
 };
 
-// Steps of kStep positions that a sequence needs, and the grain of the pieces: the same for every sequence, so that all
-// pieces are of like size however different the lengths are, and about kPieces of them over the K/V heads.
+// Steps of kStep positions that a sequence needs.
 __device__ __forceinline__ int steps_of(const FlatArgs& a, int b) {
     bool over = false;
     return b < a.B ? (held(a.kv_len[b], a.width, a.kv.shift, over) + kStep - 1) / kStep : 0;
-}
-__device__ __forceinline__ int piece_steps(const FlatArgs& a, int lane, int heads) {
-    int sum = 0;
-    for (int b0 = 0; b0 < a.B; b0 += 64) sum += __builtin_amdgcn_readlane(wave_scan(steps_of(a, b0 + lane), lane), 63);
-    const int want = max(1, kPieces / heads);
-    return max(1, (sum + want - 1) / want);
 }
 
 template <bool F16, int D>
@@ -591,16 +598,20 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_flat(const FlatA
     static_assert(sizeof(float) * 4 * 16 * OS <= sizeof(slot), "the join reuses the slots");
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 15, r = lane >> 4;
-    const int G = a.hq / a.hk, RT = (G + 15) / 16;
-    const int hr = blockIdx.x % (a.hk * RT), head = hr % a.hk, g0 = 16 * (hr / a.hk);
-    const int id = blockIdx.x / (a.hk * RT);
+    const int G = a.G;
+    const int hr = blockIdx.y, rt = a.hk == (int)gridDim.y ? 0 : hr / a.hk, head = hr - rt * a.hk, g0 = 16 * rt;
+    const int id = blockIdx.x;
 
-    // the sequence and piece of this workgroup
-    const int grain = piece_steps(a, lane, a.hk * RT);
+    // The grain of the pieces, in steps: the same for every sequence, so that all pieces are of like size however different
+    // the lengths are, and about a.want of them in all. Then the sequence and piece of this workgroup.
+    const int steps0 = steps_of(a, lane);  // of the first 64 sequences
+    int total = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 64) total += __builtin_amdgcn_readlane(wave_scan(b0 ? steps_of(a, b0 + lane) : steps0), 63);
+    const int grain = max(1, (int)(((uint32_t)total + a.want - 1) / (uint32_t)a.want));
     int b = -1, piece = 0, pieces = 0, before = 0, len = 0;
     for (int b0 = 0; b0 < a.B && b < 0; b0 += 64) {
-        const int np = (steps_of(a, b0 + lane) + grain - 1) / grain;
-        const int sum = before + wave_scan(np, lane);
+        const int np = small_div((b0 ? steps_of(a, b0 + lane) : steps0) + grain - 1, grain);
+        const int sum = before + wave_scan(np);
         const uint64_t mine = __ballot(id < sum);
         if (mine) {
             const int w = __builtin_ctzll(mine);
@@ -848,7 +859,8 @@ __global__ __launch_bounds__(256) void k_attn_join(const JoinArgs a) {
         token_range(a.cu, lo, a.T, t0, t1);
         if (tok < t0 || tok >= t1) return;
         const int rows = (t1 - t0) * G, r = (tok - t0) * G + hd % G, len = min(a.kv_own[lo], a.cap);
-        const int end = tile_end(len - (t1 - t0), rows, r / a.bm * a.bm, a.bm, G, len);
+        const int last = min(r / a.bm * a.bm + a.bm, rows) - 1;  // of the row's tile
+        const int end = max(0, len - (t1 - t0) + last / G + 1);
         nb = parts_of((end + kTile - 1) / kTile, a.nsplit, a.part_min);
         if (nb == 1) return;
     }
@@ -895,16 +907,17 @@ constexpr int rows_of(int d) { return d == 256 ? 128 : 256; }  // query rows of 
 
 template <bool F16>
 void launch_rows(const RowsArgs& a, int d, int slots, hipStream_t st) {
-    const dim3 grid((unsigned)((int64_t)slots * a.nsplit * a.hk));
+    const dim3 grid((unsigned)(a.nsplit * a.hk), (unsigned)(slots < kSlotsY ? slots : kSlotsY), (unsigned)((slots + kSlotsY - 1) / kSlotsY));
     if (d == 64) hipLaunchKernelGGL((k_attn_rows<F16, 64, 8>), grid, dim3(512), 0, st, a, slots);
     else if (d == 128) hipLaunchKernelGGL((k_attn_rows<F16, 128, 8>), grid, dim3(512), 0, st, a, slots);
     else hipLaunchKernelGGL((k_attn_rows<F16, 256, 4>), grid, dim3(256), 0, st, a, slots);
 }
 template <bool F16>
-void launch_flat(const FlatArgs& a, int d, unsigned grid, hipStream_t st) {
-    if (d == 64) hipLaunchKernelGGL((k_attn_flat<F16, 64>), dim3(grid), dim3(256), 0, st, a);
-    else if (d == 128) hipLaunchKernelGGL((k_attn_flat<F16, 128>), dim3(grid), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((k_attn_flat<F16, 256>), dim3(grid), dim3(256), 0, st, a);
+void launch_flat(const FlatArgs& a, int d, int64_t pieces, hipStream_t st) {
+    const dim3 grid((unsigned)pieces, (unsigned)(a.hk * ((a.G + 15) / 16)));
+    if (d == 64) hipLaunchKernelGGL((k_attn_flat<F16, 64>), grid, dim3(256), 0, st, a);
+    else if (d == 128) hipLaunchKernelGGL((k_attn_flat<F16, 128>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((k_attn_flat<F16, 256>), grid, dim3(256), 0, st, a);
 }
 template <bool F16>
 void launch_join(const JoinArgs& a, int d, unsigned grid, hipStream_t st) {
@@ -927,12 +940,14 @@ int row_parts(int64_t groups, int64_t positions) {
 int64_t rec_bytes(int64_t recs, int d) { return recs * (2 + d) * 4; }
 
 struct FlatWs {
+    int want;  // pieces that the grain aims at
     int64_t pieces, first, ml, po, end;
 };
 FlatWs flat_ws(int B, int hq, int hk, int d) {
     const int G = hq / hk, heads = hk * ((G + 15) / 16);
     FlatWs w;
-    w.pieces = (kPieces / heads < 1 ? 1 : kPieces / heads) + B;
+    w.want = kPieces / heads < 1 ? 1 : kPieces / heads;
+    w.pieces = w.want + B;
     w.first = 0;
     w.ml = ((int64_t)B * 8 + 15) / 16 * 16;
     w.po = w.ml + (w.pieces * hq * 8 + 15) / 16 * 16;
@@ -975,12 +990,11 @@ extern "C" int wisp_attn_prompt(const void* q, int64_t q_ts, int64_t q_hs, const
     const int bm = rows_of(d);
     const int64_t slots = row_slots(T, B, hq / hk, bm);
     const int parts = row_parts(slots * hk, (int64_t)page * width);
-    if (slots * hk * parts > 0x7FFFFFFF) return fail_inval("too many tokens for one call");
     if (parts > 1 && !ws) return fail_inval("null workspace");
     float* ml = (float*)ws;
     float* po = ml ? ml + 2 * T * hq * parts : nullptr;
     RowsArgs a{(const uint16_t*)q, q_ts, q_hs, paged_kv((void*)kc, (void*)vc, pages, page, page_stride, head_stride, row_stride),
-               cu, kv_len, table, width, B, (int)T, hq, hk, scale * 1.44269504088896340736f, parts, 4, ml, po, (uint16_t*)out};
+               cu, kv_len, table, width, B, (int)T, hq, hk, hq / hk, 1.f / (float)(hq / hk), scale * 1.44269504088896340736f, parts, 4, ml, po, (uint16_t*)out};
     hipStream_t st = (hipStream_t)stream;
     if (dtype == WISP_DT_F16) launch_rows<true>(a, d, (int)slots, st);
     else launch_rows<false>(a, d, (int)slots, st);
@@ -1020,21 +1034,21 @@ extern "C" int wisp_attn_batch(const void* q, int64_t q_ts, int64_t q_hs, const 
         return WISP_EALIGN;
     }
     const FlatWs w = flat_ws(B, hq, hk, d);
-    const int64_t blocks = w.pieces * hk * ((hq / hk + 15) / 16);
-    if (blocks > 0x7FFFFFFF || (int64_t)B * hq > (1 << 30)) return fail_inval("too many sequences for one call");
+    if ((int64_t)B * hq > (1 << 30) || (int64_t)B * ((int64_t)width * page / kStep + 1) > 0x7FFFFFFF)
+        return fail_inval("too many sequences, or positions in their tables, for one call");
     const PagedKV kv = paged_kv((void*)kc, (void*)vc, pages, page, page_stride, head_stride, row_stride);
     const float c = scale * 1.44269504088896340736f;
     uint8_t* p = (uint8_t*)ws;
     hipStream_t st = (hipStream_t)stream;
     const bool f16 = dtype == WISP_DT_F16;
-    FlatArgs f{(const uint16_t*)q, q_ts, q_hs, kv, kv_len, table, width, B, hq, hk, c, (int*)p, (float*)(p + w.ml),
+    FlatArgs f{(const uint16_t*)q, q_ts, q_hs, kv, kv_len, table, width, B, hq, hk, hq / hk, w.want, c, (int*)p, (float*)(p + w.ml),
                (float*)(p + w.po), prefix_width ? nullptr : (uint16_t*)out};
     JoinArgs j{f.first, kv_len, f.ml, f.po, nullptr, nullptr, nullptr, nullptr, 0, 1, 1, B, B, hq, hk, 0, 0, c, (uint16_t*)out};
     if (prefix_width) {
         const int bm = rows_of(d), slots = (int)(((int64_t)B * (hq / hk) + bm - 1) / bm);
         const int parts = prefix_parts(B, hq, hk, d, (int64_t)page * prefix_width);
         float* rml = (float*)(p + w.end);
-        RowsArgs a{(const uint16_t*)q, q_ts, q_hs, kv, nullptr, prefix_len, prefix_table, prefix_width, B, B, hq, hk, c, parts, 1,
+        RowsArgs a{(const uint16_t*)q, q_ts, q_hs, kv, nullptr, prefix_len, prefix_table, prefix_width, B, B, hq, hk, hq / hk, 1.f / (float)(hq / hk), c, parts, 1,
                    rml, rml + 2 * (int64_t)B * hq * parts, nullptr};
         if (f16) launch_rows<true>(a, d, slots, st);
         else launch_rows<false>(a, d, slots, st);
@@ -1043,8 +1057,8 @@ extern "C" int wisp_attn_batch(const void* q, int64_t q_ts, int64_t q_hs, const 
         j.nsplit = parts;
         j.all = 1;
     }
-    if (f16) launch_flat<true>(f, d, (unsigned)blocks, st);
-    else launch_flat<false>(f, d, (unsigned)blocks, st);
+    if (f16) launch_flat<true>(f, d, w.pieces, st);
+    else launch_flat<false>(f, d, w.pieces, st);
     if (f16) launch_join<true>(j, d, (unsigned)(B * hq), st);
     else launch_join<false>(j, d, (unsigned)(B * hq), st);
     return check_launch("k_attn_flat");
