@@ -434,7 +434,9 @@ __global__ __launch_bounds__(64 * NW, 1) void k_attn_rows(const RowsArgs a, int 
         }
     };
 
-    if constexpr (TURNS) {
+    // (one or two tiles are requested already, and are sooner done without turns)
+    const bool turns = TURNS && j1 - j0 > 2;
+    if (TURNS && turns) {
         // Interval 2j is W(j) of waves 0-3 and M(j - 1) of waves 4-7, interval 2j + 1 the other way round. In W(j) waves 0-3
         // request their part of tile j + 2 and waves 4-7 theirs of tile j + 3, whose stages' tiles j - 2 and j - 1 nobody
         // reads any more. All await tile j + 1 before interval 2j + 1, that of M(j), which is the first to read it, with one
@@ -503,7 +505,7 @@ __global__ __launch_bounds__(64 * NW, 1) void k_attn_rows(const RowsArgs a, int 
         for (int j = j0; j < j1; ++j) {
             wait_vm<0>();
             barrier();  // every wave's part of tile j is there, and nobody reads the other stage any more
-            if (j + 1 < j1) {
+            if (!TURNS && j + 1 < j1) {
                 issue(j + 1);
                 find_pages(j + 2);
             }
@@ -542,30 +544,47 @@ __global__ __launch_bounds__(64 * NW, 1) void k_attn_rows(const RowsArgs a, int 
     }
     l = add_xor32(l);
     const bool poison = bad_l != 0;
-    if (x >= t.left) return;
-    const int64_t orow = (int64_t)(t.first + tok) * a.hq + head * G + g;
+    // A lane's values lie in four-value runs of one row: through LDS, in the wave's own part of it (16-byte chunks permuted
+    // as K's), to stores of whole rows.
+    const int orow = (t.first + tok) * a.hq + head * G + g;
+    uint8_t* mine = &buf[0][0][0] + wv * (32 * 4 * D);
     if (a.out && parts == 1) {
         const float inv = poison ? __int_as_float(0x7FC00000) : l == 0.f ? 0.f : 1.f / l;
-        uint16_t* dst = a.out + orow * D + 4 * hf;
+        constexpr int SW = RB / 16 < 16 ? RB / 16 - 1 : 15;
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                *reinterpret_cast<uint2*>(dst + 32 * d + 8 * e) =
+                *reinterpret_cast<uint2*>(mine + n * RB + 16 * ((4 * d + e) ^ (n & SW)) + 8 * hf) =
                     make_uint2(pack2<F16>(o[d][4 * e] * inv, o[d][4 * e + 1] * inv),
                                pack2<F16>(o[d][4 * e + 2] * inv, o[d][4 * e + 3] * inv));
+        wait_lds();
+#pragma unroll
+        for (int i = 0; i < 32 / RPI; ++i) {
+            const int r = RPI * i + dr, to = __shfl(orow, r, 64);
+            const uint4 u = *reinterpret_cast<const uint4*>(mine + r * RB + 16 * (dc ^ (r & SW)));
+            if (32 * wv + r < t.left) *reinterpret_cast<uint4*>(a.out + (int64_t)to * D + 8 * dc) = u;
+        }
     } else {
-        const int64_t rec = orow * a.nsplit + part;
-        if (hf == 0) {
+        const int64_t rec = (int64_t)orow * a.nsplit + part;
+        if (hf == 0 && x < t.left) {
             a.ml[2 * rec] = m;
             a.ml[2 * rec + 1] = poison ? __int_as_float(0x7FC00000) : l;
         }
-        float* dst = a.po + rec * D + 4 * hf;
+        constexpr int FB = 4 * D, FPI = 1024 / FB;  // bytes of a record's row, rows per instruction
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                *reinterpret_cast<f4_t*>(dst + 32 * d + 8 * e) = f4_t{o[d][4 * e], o[d][4 * e + 1], o[d][4 * e + 2], o[d][4 * e + 3]};
+                *reinterpret_cast<f4_t*>(mine + n * FB + 16 * ((8 * d + 2 * e + hf) ^ (n & 15))) =
+                    f4_t{o[d][4 * e], o[d][4 * e + 1], o[d][4 * e + 2], o[d][4 * e + 3]};
+        wait_lds();
+#pragma unroll
+        for (int i = 0; i < 32 / FPI; ++i) {
+            const int r = FPI * i + lane / (FB / 16), fc = lane % (FB / 16), to = __shfl(orow, r, 64);
+            const f4_t u = *reinterpret_cast<const f4_t*>(mine + r * FB + 16 * (fc ^ (r & 15)));
+            if (32 * wv + r < t.left) *reinterpret_cast<f4_t*>(a.po + ((int64_t)to * a.nsplit + part) * D + 4 * fc) = u;
+        }
     }
 }
 
