@@ -43,7 +43,7 @@ constexpr int kSub = 32;           // positions per slot of k_attn_flat
 constexpr int kStep = 4 * kSub;    // positions of a workgroup's four slots: the grain of its pieces
 constexpr float kLazy = 6.f;       // m follows the maximum past 2^kLazy
 constexpr int kSlotsY = 32768;     // grid.y of k_attn_rows
-constexpr int kPieces = 1024;      // pieces that k_attn_flat aims at over all sequences and K/V heads
+constexpr int kMaxParts = 64;       // parts of a shared prefix
 
 // float16 weights p: times 2^8, so that small ones keep their bits (the grain 2^-24 is then 2^-32 of the largest) and
 // 2^(8 + kLazy) stays below the type's 65,504. bfloat16 has binary32's range.
@@ -598,6 +598,9 @@ struct FlatArgs {
     float c;
     int* first;      // [B][2]: number of the sequence's first piece, its pieces
     float *ml, *po;  // records [(first + piece) * hq + head]
+    const float *rml, *rpo;  // with a prefix: its records [(b * hq + head) * nsplit + part]
+    int nsplit;
+    int single;      // every sequence is one piece, and what this kernel leaves is the result
     uint16_t* out;   // [B][hq][D]; null: every piece leaves a record (a prefix's are to be added)
 };
 
@@ -621,35 +624,38 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_flat(const FlatA
     const int hr = blockIdx.y, rt = a.hk == (int)gridDim.y ? 0 : hr / a.hk, head = hr - rt * a.hk, g0 = 16 * rt;
     const int id = blockIdx.x;
 
-    // The grain of the pieces, in steps: the same for every sequence, so that all pieces are of like size however different
-    // the lengths are, and about a.want of them in all. Then the sequence and piece of this workgroup.
-    const int steps0 = steps_of(a, lane);  // of the first 64 sequences
-    int total = 0;
-    for (int b0 = 0; b0 < a.B; b0 += 64) total += __builtin_amdgcn_readlane(wave_scan(b0 ? steps_of(a, b0 + lane) : steps0), 63);
-    const int grain = max(1, (int)(((uint32_t)total + a.want - 1) / (uint32_t)a.want));
-    int b = -1, piece = 0, pieces = 0, before = 0, len = 0;
-    for (int b0 = 0; b0 < a.B && b < 0; b0 += 64) {
-        const int np = small_div((b0 ? steps_of(a, b0 + lane) : steps0) + grain - 1, grain);
-        const int sum = before + wave_scan(np);
-        const uint64_t mine = __ballot(id < sum);
-        if (mine) {
-            const int w = __builtin_ctzll(mine);
-            b = b0 + w;
-            pieces = __builtin_amdgcn_readlane(np, w);
-            before = __builtin_amdgcn_readlane(sum, w) - pieces;
-            piece = id - before;
-        } else {
-            before = __builtin_amdgcn_readlane(sum, 63);
+    int b = id, piece = 0, pieces = 1, before = 0, grain = 1 << 23;
+    if (!a.single) {
+        // The grain of the pieces, in steps: the same for every sequence, so that all pieces are of like size however
+        // different the lengths are, and no more than a.want of them in all, if it can be. Then this workgroup's.
+        const int steps0 = steps_of(a, lane);  // of the first 64 sequences
+        int total = 0;
+        for (int b0 = 0; b0 < a.B; b0 += 64) total += __builtin_amdgcn_readlane(wave_scan(b0 ? steps_of(a, b0 + lane) : steps0), 63);
+        grain = max(1, (int)(((uint32_t)total + a.want - 1) / (uint32_t)a.want));
+        b = -1;
+        for (int b0 = 0; b0 < a.B && b < 0; b0 += 64) {
+            const int np = small_div((b0 ? steps_of(a, b0 + lane) : steps0) + grain - 1, grain);
+            const int sum = before + wave_scan(np);
+            const uint64_t mine = __ballot(id < sum);
+            if (mine) {
+                const int w = __builtin_ctzll(mine);
+                b = b0 + w;
+                pieces = __builtin_amdgcn_readlane(np, w);
+                before = __builtin_amdgcn_readlane(sum, w) - pieces;
+                piece = id - before;
+            } else {
+                before = __builtin_amdgcn_readlane(sum, 63);
+            }
+        }
+        if (b < 0) return;
+        if (piece == 0 && hr == 0 && threadIdx.x == 0) {
+            a.first[2 * b] = before;
+            a.first[2 * b + 1] = pieces;
         }
     }
-    if (b < 0) return;
     bool bad = false;
-    len = held(scalar_at(a.kv_len, b), a.width, a.kv.shift, bad);
-    if (piece == 0 && hr == 0 && threadIdx.x == 0) {
-        a.first[2 * b] = before;
-        a.first[2 * b + 1] = pieces;
-    }
-    const int from = piece * grain * kStep, to = min(len, from + grain * kStep);
+    const int len = held(scalar_at(a.kv_len, b), a.width, a.kv.shift, bad);
+    const int from = piece * grain * kStep, to = (int)min((int64_t)len, from + (int64_t)grain * kStep);
 
     const int* trow = a.table + (int64_t)b * a.width;
     const uint8_t* kbase = a.kv.kc + head * a.kv.hs;
@@ -809,10 +815,73 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_flat(const FlatA
     for (int d = 0; d < ND; ++d)
         *reinterpret_cast<f4_t*>(join + (wv * 16 + n) * OS + 16 * d + 4 * r) = f4_t{o[d][0] * f, o[d][1] * f, o[d][2] * f, o[d][3] * f};
     barrier();
-    const bool whole = a.out && pieces == 1;
-    for (int e = threadIdx.x; e < min(16, G - g0) * (D / 2); e += 256) {
+    const int rows = min(16, G - g0);
+    const int64_t row0 = (int64_t)b * a.hq + head * G + g0;  // of out
+    const int parts = a.single ? a.nsplit : 0;
+    // This piece's share of each row, and those of the prefix's parts, as factors of their O, 1/L of the whole included:
+    // 16 lanes a row.
+    __shared__ float own[16], share[16][kMaxParts];
+    if (parts) {
+        const int row = min((int)threadIdx.x >> 4, rows - 1), e = threadIdx.x & 15;
+        float Mr = red[0][row][0], L = 0.f;
+#pragma unroll
+        for (int w = 1; w < 4; ++w) Mr = fmaxf(Mr, red[w][row][0]);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) L += red[w][row][0] == -INFINITY ? red[w][row][1] : red[w][row][1] * __builtin_amdgcn_exp2f((red[w][row][0] - Mr) * c);
+        float m[kMaxParts / 16], ll[kMaxParts / 16], Mx = Mr;
+#pragma unroll
+        for (int k = 0; k < kMaxParts / 16; ++k) {
+            const int p = e + 16 * k;
+            m[k] = p < parts ? a.rml[2 * ((row0 + row) * parts + p)] : -INFINITY;
+            ll[k] = p < parts ? a.rml[2 * ((row0 + row) * parts + p) + 1] : 0.f;
+            Mx = fmaxf(Mx, m[k]);
+        }
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) Mx = fmaxf(Mx, __shfl_xor(Mx, o, 64));
+        float sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < kMaxParts / 16; ++k) {
+            const float w = m[k] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m[k] - Mx) * c);
+            sum += m[k] == -INFINITY ? ll[k] : ll[k] * w;  // (a record without weights has m = -inf; its l may be a bad page's NaN)
+            m[k] = w;
+        }
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) sum += __shfl_xor(sum, o, 64);
+        const float f0 = Mr == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((Mr - Mx) * c);
+        sum += Mr == -INFINITY ? L : L * f0;
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        if ((int)threadIdx.x >> 4 < rows) {
+            if (e == 0) own[row] = f0 * inv;
+#pragma unroll
+            for (int k = 0; k < kMaxParts / 16; ++k)
+                if (e + 16 * k < parts) share[row][e + 16 * k] = m[k] * inv;
+        }
+        __syncthreads();
+    }
+    for (int e = threadIdx.x; e < rows * (D / 2); e += 256) {
         const int row = e / (D / 2), d = 2 * (e - row * (D / 2));
-        float Mr = red[0][row][0], L = 0.f, x = 0.f, y = 0.f;
+        float x = 0.f, y = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            x += join[(w * 16 + row) * OS + d];
+            y += join[(w * 16 + row) * OS + d + 1];
+        }
+        uint16_t* const to_out = a.out + (row0 + row) * D + d;
+        if (parts) {
+            x *= own[row];
+            y *= own[row];
+            const float* po = a.rpo + (row0 + row) * parts * D + d;
+#pragma unroll 8
+            for (int p = 0; p < parts; ++p) {
+                const float f = share[row][p];
+                const float2 v = *reinterpret_cast<const float2*>(po + p * D);
+                x += f == 0.f ? 0.f : f * v.x;  // (the O of a record without weights is zeros, or of NaN values that have none)
+                y += f == 0.f ? 0.f : f * v.y;
+            }
+            *reinterpret_cast<uint32_t*>(to_out) = pack2<F16>(x, y);
+            continue;
+        }
+        float Mr = red[0][row][0], L = 0.f;
 #pragma unroll
         for (int w = 1; w < 4; ++w) Mr = fmaxf(Mr, red[w][row][0]);
 #pragma unroll
@@ -820,14 +889,12 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_flat(const FlatA
             const float mw = red[w][row][0], lw = red[w][row][1];
             // (a wave without positions has m = -inf and l = 0, or NaN from a bad page)
             L += mw == -INFINITY ? lw : lw * __builtin_amdgcn_exp2f((mw - Mr) * c);
-            x += join[(w * 16 + row) * OS + d];
-            y += join[(w * 16 + row) * OS + d + 1];
         }
-        const int hd = head * G + g0 + row;
-        if (whole) {
-            *reinterpret_cast<uint32_t*>(a.out + ((int64_t)b * a.hq + hd) * D + d) = pack2<F16>(x / L, y / L);
+        if (a.out && pieces == 1) {
+            const float inv = L == 0.f ? 0.f : 1.f / L;
+            *reinterpret_cast<uint32_t*>(to_out) = pack2<F16>(x * inv, y * inv);
         } else {
-            const int64_t rec = (int64_t)(before + piece) * a.hq + hd;
+            const int64_t rec = (int64_t)(before + piece) * a.hq + head * G + g0 + row;
             if (d == 0) {
                 a.ml[2 * rec] = Mr;
                 a.ml[2 * rec + 1] = L;
@@ -933,7 +1000,7 @@ void launch_rows(const RowsArgs& a, int d, int slots, hipStream_t st) {
 }
 template <bool F16>
 void launch_flat(const FlatArgs& a, int d, int64_t pieces, hipStream_t st) {
-    const dim3 grid((unsigned)pieces, (unsigned)(a.hk * ((a.G + 15) / 16)));
+    const dim3 grid((unsigned)(a.single ? a.B : pieces), (unsigned)(a.hk * ((a.G + 15) / 16)));
     if (d == 64) hipLaunchKernelGGL((k_attn_flat<F16, 64>), grid, dim3(256), 0, st, a);
     else if (d == 128) hipLaunchKernelGGL((k_attn_flat<F16, 128>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((k_attn_flat<F16, 256>), grid, dim3(256), 0, st, a);
@@ -949,11 +1016,19 @@ void launch_join(const JoinArgs& a, int d, unsigned grid, hipStream_t st) {
 int64_t row_slots(int64_t T, int B, int G, int bm) { return (T * G + bm - 1) / bm + B - 1; }
 
 // Parts for each row tile: where the tiles alone leave CUs without work and the positions are many, enough to occupy the
-// card once (256 CUs, one workgroup each), but at least 4 tiles of positions each.
+// card once (256 CUs, one workgroup each), but at least kPartTiles tiles of positions each.
+constexpr int kPartTiles = 2;
 int row_parts(int64_t groups, int64_t positions) {
-    const int64_t most = (positions + kTile - 1) / kTile / 4;
+    const int64_t most = (positions + kTile - 1) / kTile / kPartTiles;
     const int64_t want = groups < 1 ? 1 : 256 / groups;
     return (int)(want < most ? (want < 1 ? 1 : want) : (most < 1 ? 1 : most));
+}
+
+// Whether k_attn_flat takes each sequence whole, which spares the records and k_attn_join: where no table holds more than
+// 4 steps of positions, or 8 where there are workgroups enough without pieces, or a prefix's records to be added anyway.
+bool takes_whole(int B, int hq, int hk, int64_t positions, bool prefix) {
+    const int64_t groups = (int64_t)B * hk * ((hq / hk + 15) / 16);
+    return positions <= (groups >= 256 || prefix ? 8 : 4) * kStep;
 }
 
 int64_t rec_bytes(int64_t recs, int d) { return recs * (2 + d) * 4; }
@@ -962,10 +1037,11 @@ struct FlatWs {
     int want;  // pieces that the grain aims at
     int64_t pieces, first, ml, po, end;
 };
+// k_attn_flat's pieces: as many as workgroups that 256 CUs hold at once (their LDS: 4, 2 or 1 a CU).
 FlatWs flat_ws(int B, int hq, int hk, int d) {
-    const int G = hq / hk, heads = hk * ((G + 15) / 16);
+    const int G = hq / hk, heads = hk * ((G + 15) / 16), most = d == 64 ? 1024 : d == 128 ? 512 : 256;
     FlatWs w;
-    w.want = kPieces / heads < 1 ? 1 : kPieces / heads;
+    w.want = most / heads < 1 ? 1 : most / heads;
     w.pieces = w.want + B;
     w.first = 0;
     w.ml = ((int64_t)B * 8 + 15) / 16 * 16;
@@ -1013,12 +1089,12 @@ extern "C" int wisp_attn_prompt(const void* q, int64_t q_ts, int64_t q_hs, const
     float* ml = (float*)ws;
     float* po = ml ? ml + 2 * T * hq * parts : nullptr;
     RowsArgs a{(const uint16_t*)q, q_ts, q_hs, paged_kv((void*)kc, (void*)vc, pages, page, page_stride, head_stride, row_stride),
-               cu, kv_len, table, width, B, (int)T, hq, hk, hq / hk, 1.f / (float)(hq / hk), scale * 1.44269504088896340736f, parts, 4, ml, po, (uint16_t*)out};
+               cu, kv_len, table, width, B, (int)T, hq, hk, hq / hk, 1.f / (float)(hq / hk), scale * 1.44269504088896340736f, parts, kPartTiles, ml, po, (uint16_t*)out};
     hipStream_t st = (hipStream_t)stream;
     if (dtype == WISP_DT_F16) launch_rows<true>(a, d, (int)slots, st);
     else launch_rows<false>(a, d, (int)slots, st);
     if (parts > 1) {
-        JoinArgs j{nullptr, nullptr, nullptr, nullptr, cu, kv_len, ml, po, parts, 4, bm, B, (int)T, hq, hk, width * page, 0, a.c, (uint16_t*)out};
+        JoinArgs j{nullptr, nullptr, nullptr, nullptr, cu, kv_len, ml, po, parts, kPartTiles, bm, B, (int)T, hq, hk, width * page, 0, a.c, (uint16_t*)out};
         if (dtype == WISP_DT_F16) launch_join<true>(j, d, (unsigned)(T * hq), st);
         else launch_join<false>(j, d, (unsigned)(T * hq), st);
     }
@@ -1028,7 +1104,8 @@ extern "C" int wisp_attn_prompt(const void* q, int64_t q_ts, int64_t q_hs, const
 // The parts of a shared prefix: rows of all B sequences together.
 static int prefix_parts(int B, int hq, int hk, int d, int64_t positions) {
     const int bm = rows_of(d);
-    return row_parts((int64_t)(((int64_t)B * (hq / hk) + bm - 1) / bm) * hk, positions);
+    const int n = row_parts((int64_t)(((int64_t)B * (hq / hk) + bm - 1) / bm) * hk, positions);
+    return n < kMaxParts ? n : kMaxParts;
 }
 
 extern "C" int64_t wisp_attn_batch_ws_bytes(int B, int hq, int hk, int d, int page, int prefix_width) {
@@ -1061,7 +1138,8 @@ extern "C" int wisp_attn_batch(const void* q, int64_t q_ts, int64_t q_hs, const 
     hipStream_t st = (hipStream_t)stream;
     const bool f16 = dtype == WISP_DT_F16;
     FlatArgs f{(const uint16_t*)q, q_ts, q_hs, kv, kv_len, table, width, B, hq, hk, hq / hk, w.want, c, (int*)p, (float*)(p + w.ml),
-               (float*)(p + w.po), prefix_width ? nullptr : (uint16_t*)out};
+               (float*)(p + w.po), nullptr, nullptr, 0, takes_whole(B, hq, hk, (int64_t)width * page, prefix_width > 0), (uint16_t*)out};
+    if (prefix_width && !f.single) f.out = nullptr;
     JoinArgs j{f.first, kv_len, f.ml, f.po, nullptr, nullptr, nullptr, nullptr, 0, 1, 1, B, B, hq, hk, 0, 0, c, (uint16_t*)out};
     if (prefix_width) {
         const int bm = rows_of(d), slots = (int)(((int64_t)B * (hq / hk) + bm - 1) / bm);
@@ -1071,14 +1149,16 @@ extern "C" int wisp_attn_batch(const void* q, int64_t q_ts, int64_t q_hs, const 
                    rml, rml + 2 * (int64_t)B * hq * parts, nullptr};
         if (f16) launch_rows<true>(a, d, slots, st);
         else launch_rows<false>(a, d, slots, st);
-        j.rml = a.ml;
-        j.rpo = a.po;
-        j.nsplit = parts;
+        j.rml = f.rml = a.ml;
+        j.rpo = f.rpo = a.po;
+        j.nsplit = f.nsplit = parts;
         j.all = 1;
     }
     if (f16) launch_flat<true>(f, d, w.pieces, st);
     else launch_flat<false>(f, d, w.pieces, st);
-    if (f16) launch_join<true>(j, d, (unsigned)(B * hq), st);
-    else launch_join<false>(j, d, (unsigned)(B * hq), st);
+    if (!f.single) {
+        if (f16) launch_join<true>(j, d, (unsigned)(B * hq), st);
+        else launch_join<false>(j, d, (unsigned)(B * hq), st);
+    }
     return check_launch("k_attn_flat");
 }
