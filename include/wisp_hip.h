@@ -253,8 +253,8 @@ int wisp_attn_prompt(const void* q, int64_t q_ts, int64_t q_hs, const void* kc, 
 /* One token of each sequence: out [B][hq][d] over the kv_len[b] positions of b (none: zeros). With prefix_width > 0 every
  * sequence first attends the prefix_len[0] positions of prefix_table [prefix_width] (device int32), read once for all of
  * them; kv_len and table are then what each sequence has of its own. ws: wisp_attn_batch_ws_bytes(B, hq, hk, d, page,
- * prefix_width) bytes, 16-byte aligned. */
-int64_t wisp_attn_batch_ws_bytes(int B, int hq, int hk, int d, int page, int prefix_width);
+ * width, prefix_width) bytes, 16-byte aligned (may be NULL where that is 0). */
+int64_t wisp_attn_batch_ws_bytes(int B, int hq, int hk, int d, int page, int width, int prefix_width);
 int wisp_attn_batch(const void* q, int64_t q_ts, int64_t q_hs, const void* kc, const void* vc, int64_t pages, int page,
                     int64_t page_stride, int64_t head_stride, int64_t row_stride, const int32_t* kv_len,
                     const int32_t* table, int width, const int32_t* prefix_len, const int32_t* prefix_table,

@@ -75,7 +75,8 @@ def test_cache_alignment(call, args):
     (_prompt, dict(scale=-1.0), b"scale"), (_prompt, dict(scale=float("inf")), b"scale"),
     (_prompt, dict(scale=float("nan")), b"scale"), (_prompt, dict(out=None), b"null"), (_prompt, dict(cu=None), b"null"),
     (_prompt, dict(ws=None, width=400), b"workspace"),
-    (_batch, dict(scale=0.0), b"scale"), (_batch, dict(ws=None), b"null"), (_batch, dict(prefix_len=None), b"null"),
+    (_batch, dict(scale=0.0), b"scale"), (_batch, dict(ws=None), b"workspace"),
+    (_batch, dict(ws=None, prefix_width=0, width=400), b"workspace"), (_batch, dict(prefix_len=None), b"null"),
     (_batch, dict(prefix_width=-1), b"prefix"), (_batch, dict(prefix_width=1 << 28), b"prefix"),
     (_batch, dict(kv_len=None), b"null"),
 ])
@@ -102,9 +103,11 @@ def test_workspaces():
     assert L.wisp_attn_prompt_ws_bytes(0, 1, 32, 4, 128, 64, 256) == 0
     assert L.wisp_attn_prompt_ws_bytes(8, 1, 32, 4, 128, 64, 256) > 0
     assert L.wisp_attn_prompt_ws_bytes(8, 1, 30, 4, 128, 64, 256) == -1
-    assert L.wisp_attn_batch_ws_bytes(0, 32, 4, 128, 64, 0) == -1
-    own = L.wisp_attn_batch_ws_bytes(8, 32, 4, 128, 64, 0)
-    assert 0 < own < L.wisp_attn_batch_ws_bytes(8, 32, 4, 128, 64, 256)
+    assert L.wisp_attn_batch_ws_bytes(0, 32, 4, 128, 64, 99, 0) == -1
+    assert L.wisp_attn_batch_ws_bytes(8, 32, 4, 128, 64, 0, 0) == -1
+    assert L.wisp_attn_batch_ws_bytes(8, 32, 4, 128, 64, 2, 0) == 0  # short tables: no pieces, no records
+    own = L.wisp_attn_batch_ws_bytes(8, 32, 4, 128, 64, 99, 0)
+    assert 0 < own < L.wisp_attn_batch_ws_bytes(8, 32, 4, 128, 64, 99, 256)
 
 
 def test_cpu_tensors_and_wrong_types_are_refused():

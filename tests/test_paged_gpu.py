@@ -440,6 +440,9 @@ BATCH = [
     (HF, 3, 3, 256, 32, "hnd", [64, 65, 66]),
     (BF, 8, 2, 128, 16, "hnd", [(37 * i) % 300 for i in range(150)]),
     (BF, 8, 1, 64, 64, "hnd", [70000]),
+    (BF, 32, 4, 128, 64, "hnd", [200, 0, 512, 7]),  # short tables: taken whole
+    (HF, 20, 1, 64, 16, "nhd", [(13 * i) % 500 for i in range(130)]),
+    (HF, 16, 2, 256, 64, "hnd", [1025, 0, 3000]),
 ]
 
 
@@ -458,6 +461,9 @@ SHARED = [
     (BF, 16, 2, 256, 16, "nhd", 333, [20, 1]),
     (HF, 40, 8, 128, 128, "gaps", 64, [(11 * i) % 130 for i in range(70)]),
     (BF, 7, 1, 128, 64, "hnd", 5000, [10, 0, 300]),
+    (BF, 32, 4, 128, 64, "hnd", 900, [1500, 0, 3]),  # own tables past what is taken whole
+    (HF, 20, 1, 64, 32, "hnd", 9000, [2000, 5]),
+    (HF, 16, 2, 256, 16, "hnd", 2000, [1100, 0, 64, 9]),
 ]
 
 

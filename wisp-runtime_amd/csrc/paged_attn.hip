@@ -1108,9 +1108,10 @@ static int prefix_parts(int B, int hq, int hk, int d, int64_t positions) {
     return n < kMaxParts ? n : kMaxParts;
 }
 
-extern "C" int64_t wisp_attn_batch_ws_bytes(int B, int hq, int hk, int d, int page, int prefix_width) {
-    if (B < 1 || hk < 1 || hq < hk || hq % hk || d < 64 || page < 1 || prefix_width < 0) return -1;
-    const int64_t own = flat_ws(B, hq, hk, d).end;
+extern "C" int64_t wisp_attn_batch_ws_bytes(int B, int hq, int hk, int d, int page, int width, int prefix_width) {
+    if (B < 1 || hk < 1 || hq < hk || hq % hk || d < 64 || page < 1 || width < 1 || prefix_width < 0) return -1;
+    const bool whole = takes_whole(B, hq, hk, (int64_t)width * page, prefix_width > 0);
+    const int64_t own = whole ? 0 : flat_ws(B, hq, hk, d).end;
     return prefix_width ? own + rec_bytes((int64_t)B * hq * prefix_parts(B, hq, hk, d, (int64_t)page * prefix_width), d) : own;
 }
 
@@ -1123,13 +1124,16 @@ extern "C" int wisp_attn_batch(const void* q, int64_t q_ts, int64_t q_hs, const 
     if (int rc = check_paged(kc, vc, pages, page, page_stride, head_stride, row_stride, width, B, hq, hk, d, dtype)) return rc;
     if (!good_scale(scale)) return fail_inval("scale must be positive and finite");
     if (prefix_width < 0 || (int64_t)prefix_width * page > (1 << 30)) return fail_inval("the prefix's positions must be in [0, 2^30]");
-    if (!q || !kv_len || !table || !out || !ws || (prefix_width && (!prefix_len || !prefix_table))) return fail_inval("null pointer");
+    if (!q || !kv_len || !table || !out || (prefix_width && (!prefix_len || !prefix_table))) return fail_inval("null pointer");
+    const bool whole = takes_whole(B, hq, hk, (int64_t)width * page, prefix_width > 0);
+    if (!ws && (!whole || prefix_width)) return fail_inval("null workspace");
     if (int rc = check_q(q, q_ts, q_hs, out)) return rc;
     if (!aligned(ws, 16)) {
         set_error("ws must be 16-byte aligned");
         return WISP_EALIGN;
     }
-    const FlatWs w = flat_ws(B, hq, hk, d);
+    FlatWs w = flat_ws(B, hq, hk, d);
+    if (whole) w.ml = w.po = w.end = 0;  // (no records of its own)
     if ((int64_t)B * hq > (1 << 30) || (int64_t)B * ((int64_t)width * page / kStep + 1) > 0x7FFFFFFF)
         return fail_inval("too many sequences, or positions in their tables, for one call");
     const PagedKV kv = paged_kv((void*)kc, (void*)vc, pages, page, page_stride, head_stride, row_stride);
@@ -1138,7 +1142,7 @@ extern "C" int wisp_attn_batch(const void* q, int64_t q_ts, int64_t q_hs, const 
     hipStream_t st = (hipStream_t)stream;
     const bool f16 = dtype == WISP_DT_F16;
     FlatArgs f{(const uint16_t*)q, q_ts, q_hs, kv, kv_len, table, width, B, hq, hk, hq / hk, w.want, c, (int*)p, (float*)(p + w.ml),
-               (float*)(p + w.po), nullptr, nullptr, 0, takes_whole(B, hq, hk, (int64_t)width * page, prefix_width > 0), (uint16_t*)out};
+               (float*)(p + w.po), nullptr, nullptr, 0, whole, (uint16_t*)out};
     if (prefix_width && !f.single) f.out = nullptr;
     JoinArgs j{f.first, kv_len, f.ml, f.po, nullptr, nullptr, nullptr, nullptr, 0, 1, 1, B, B, hq, hk, 0, 0, c, (uint16_t*)out};
     if (prefix_width) {

@@ -65,7 +65,7 @@ SIGNATURES = {
     "wisp_attn_prompt_ws_bytes": (_i64, [_i64, _i32, _i32, _i32, _i32, _i32, _i32]),
     "wisp_attn_prompt": (_i32, [_vp, _i64, _i64, _vp, _vp, _i64, _i32, _i64, _i64, _i64, _vp, _vp, _vp, _i32, _i32, _i64,
                                 _i32, _i32, _i32, _i32, ctypes.c_float, _vp, _vp, _vp]),
-    "wisp_attn_batch_ws_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32, _i32]),
+    "wisp_attn_batch_ws_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32, _i32, _i32]),
     "wisp_attn_batch": (_i32, [_vp, _i64, _i64, _vp, _vp, _i64, _i32, _i64, _i64, _i64, _vp, _vp, _i32, _vp, _vp, _i32,
                                _i32, _i32, _i32, _i32, _i32, ctypes.c_float, _vp, _vp, _vp]),
     "wisp_core_create": (_i32, [_i64, _i32, _f64, _i64, _f64, _vp]),

@@ -584,7 +584,7 @@ def _rows(x, what):
 
 def _out(out, shape, like):
     if out is None:
-        return torch.empty(shape, dtype=like.dtype, device=like.device)
+        return torch.empty_like(like) if like.is_contiguous() else torch.empty(shape, dtype=like.dtype, device=like.device)
     assert out.shape == shape and out.dtype == like.dtype and out.is_contiguous(), f"out must be a contiguous {shape} tensor"
     assert out.device == like.device
     return out
@@ -680,11 +680,11 @@ def _attn_batch(q, kc, vc, kv_len, table, prefix, scale, out, what):
     q, qp, q_ts, q_hs = _rows(q, "q")
     out = _out(out, (B, hq, D), q)
     L = _lib.lib()
-    nb = L.wisp_attn_batch_ws_bytes(B, hq, hk, D, cache[3], pre[2])
-    ws = torch.empty(max(nb, 0), dtype=torch.uint8, device=dev)
+    nb = L.wisp_attn_batch_ws_bytes(B, hq, hk, D, cache[3], width, pre[2])
+    ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb > 0 else None
     _call(dev, L.wisp_attn_batch,
-          (qp, q_ts, q_hs, *cache, kv_len.data_ptr(), table.data_ptr(), width, *pre, B, hq, hk, D, dt, scale, ws.data_ptr(),
-           out.data_ptr()), what)
+          (qp, q_ts, q_hs, *cache, kv_len.data_ptr(), table.data_ptr(), width, *pre, B, hq, hk, D, dt, scale,
+           None if ws is None else ws.data_ptr(), out.data_ptr()), what)
     return out
 
 
