@@ -40,7 +40,8 @@ How this build lays it out:
     step; the cache copies its state back to the host core when the host next needs it.
   * Prefill runs the model's own modules over chunks of tokens, attention in float32 over
     the static cache with the KV heads repeated for their query groups; K/V are written
-    straight into the static buffers.
+    straight into the static buffers. With fused=True the part between the projections is
+    kv_append and attn_prompt, the static cache seen as pages of 64 positions.
 """
 
 from __future__ import annotations
@@ -189,10 +190,13 @@ class GraphDecoder:
 
     # ---------------------------------------------------------------- prefill
     @torch.no_grad()
-    def prefill(self, ids, start=None, chunk=1024):
+    def prefill(self, ids, start=None, chunk=1024, fused=False):
         """Run tokens `ids` ([T]) at positions start .. start+T-1 through the model's modules
         and the paged MoE blocks, writing K/V into the static buffers (positions before
-        `start` are kept and attended). Returns the logits [1, V] of the last token."""
+        `start` are kept and attended). Returns the logits [1, V] of the last token.
+        fused: head norms, rotation, the K/V store and attention by kernels.kv_append and
+        kernels.attn_prompt over the static buffers (two or three launches a layer) instead of
+        the modules and a float32 attention; results differ by bf16 rounding."""
         from transformers.models.qwen3_moe.modeling_qwen3_moe import apply_rotary_pos_emb
 
         start = self.pos if start is None else start
@@ -206,13 +210,24 @@ class GraphDecoder:
             toks = ids[c0 : c0 + chunk]
             T, s0 = toks.numel(), start + c0
             s1 = s0 + T
-            cos, sin = self.cos[s0:s1][None], self.sin[s0:s1][None]
-            # query s0 + t sees keys 0 .. s0 + t
-            causal = torch.arange(s1, device=self.dev)[None, :] <= torch.arange(s0, s1, device=self.dev)[:, None]
             h = embed(toks.view(1, T))
+            if fused:
+                # the static buffers as a paged cache: pages of 64 positions, in order
+                cu = torch.tensor([0, T], dtype=torch.int32, device=self.dev)
+                kv_len = torch.tensor([s1], dtype=torch.int32, device=self.dev)
+                table = torch.arange((self.tmax + SCRATCH) // 64, dtype=torch.int32, device=self.dev)[None]
+            else:
+                cos, sin = self.cos[s0:s1][None], self.sin[s0:s1][None]
+                # query s0 + t sees keys 0 .. s0 + t
+                causal = torch.arange(s1, device=self.dev)[None, :] <= torch.arange(s0, s1, device=self.dev)[:, None]
             for i, lay in enumerate(self.layers):
                 at = lay.self_attn
                 xn = lay.input_layernorm(h)
+                if fused:
+                    h = h + at.o_proj(self._attend_fused(i, at, xn, cu, kv_len, table).view(1, T, Hq * D))
+                    y = lay.mlp(lay.post_attention_layernorm(h))
+                    h = h + (y[0] if isinstance(y, tuple) else y)
+                    continue
                 q = at.q_norm(at.q_proj(xn).view(1, T, Hq, D)).transpose(1, 2)
                 kk = at.k_norm(at.k_proj(xn).view(1, T, Hk, D)).transpose(1, 2)
                 vv = at.v_proj(xn).view(1, T, Hk, D).transpose(1, 2)
@@ -230,6 +245,15 @@ class GraphDecoder:
             logits = head(final(h[:, -1:])).view(1, -1)
         self.pos = total
         return logits
+
+    def _attend_fused(self, i, at, xn, cu, kv_len, table):
+        """Attention [T, Hq, D] of layer i's normed input xn over the static buffers, its K/V stored there."""
+        w, D = self.shape.per_layer[i], self.D
+        q, k, v = (proj(xn).view(-1, heads, D) for proj, heads in ((at.q_proj, self.Hq), (at.k_proj, self.Hk),
+                                                                   (at.v_proj, self.Hk)))
+        kc, vc = (self.kv[i, j].view(self.Hk, -1, 64, D).transpose(0, 1) for j in range(2))
+        q = kernels.kv_append(q, k, v, self.cos, self.sin, cu, kv_len, table, kc, vc, w["qn"], w["kn"], w["epsq"])
+        return kernels.attn_prompt(q, kc, vc, cu, kv_len, table, w["scale"])
 
     # ---------------------------------------------------------------- segment bodies
     def _attention_router(self, i, a, a_row=None, b=None):
