@@ -278,6 +278,8 @@ PROMPT = [
     (BF, 4, 4, 64, 64, "hnd", [300], [0]),
     (BF, 40, 8, 128, 64, "hnd", [10, 12], [-4, -12]),
     (HF, 24, 1, 128, 64, "hnd", [33], [64]),
+    (BF, 64, 16, 64, 64, "hnd", [700, 0, 641], [0, 10, 3]),  # many rows of 64: four waves a workgroup
+    (HF, 36, 18, 64, 32, "nhd", [2300], [0]),
 ]
 
 

@@ -238,7 +238,7 @@ __device__ __forceinline__ bool find_tile(const RowsArgs& a, int s, int lane, Ro
 // a barrier swaps the parts. A turn M(j) is O += V(j) P(j), then S(j + 1) = K(j + 1) Q^T; a turn W(j) turns S(j) into
 // P(j). K and V of four tiles are in LDS or on their way.
 template <bool F16, int D, int NW>
-__global__ __launch_bounds__(64 * NW, 1) void k_attn_rows(const RowsArgs a, int slots) {
+__global__ __launch_bounds__(64 * NW, D == 64 && NW == 4 ? 3 : 1) void k_attn_rows(const RowsArgs a, int slots) {
     constexpr int BM = 32 * NW, KD = D / 16, ND = D / 32, RB = 2 * D;  // RB: bytes of a row
     constexpr int RPI = 1024 / RB;                                      // rows per load instruction
     constexpr int LPW = kTile / RPI / NW;                               // K (and V) load instructions per wave and tile
@@ -989,12 +989,17 @@ __global__ __launch_bounds__(256) void k_attn_join(const JoinArgs a) {
 }
 
 // ---------------------------------------------------------------------------
-constexpr int rows_of(int d) { return d == 256 ? 128 : 256; }  // query rows of a k_attn_rows workgroup
+// Query rows of a k_attn_rows workgroup. D = 256: four waves, whose registers the CU's whole file holds. D = 128: eight.
+// D = 64, where a tile's weights cost twice its matrix products: four waves, four workgroups to a CU,
+// where there are enough to keep them all busy (64 query and 8 K/V heads, 4,000 tokens: 164 -> 150 us; 1,500 in three
+// prompts: 28.4 -> 26.3), else eight waves that take turns (1,018 tokens behind 24,000: 399 us, 428 with four).
+int rows_of(int d, int64_t rows, int hk) { return d == 256 || (d == 64 && rows / 128 * hk >= 640) ? 128 : 256; }
 
 template <bool F16>
-void launch_rows(const RowsArgs& a, int d, int slots, hipStream_t st) {
+void launch_rows(const RowsArgs& a, int d, int bm, int slots, hipStream_t st) {
     const dim3 grid((unsigned)(a.nsplit * a.hk), (unsigned)(slots < kSlotsY ? slots : kSlotsY), (unsigned)((slots + kSlotsY - 1) / kSlotsY));
-    if (d == 64) hipLaunchKernelGGL((k_attn_rows<F16, 64, 8>), grid, dim3(512), 0, st, a, slots);
+    if (d == 64 && bm == 128) hipLaunchKernelGGL((k_attn_rows<F16, 64, 4>), grid, dim3(256), 0, st, a, slots);
+    else if (d == 64) hipLaunchKernelGGL((k_attn_rows<F16, 64, 8>), grid, dim3(512), 0, st, a, slots);
     else if (d == 128) hipLaunchKernelGGL((k_attn_rows<F16, 128, 8>), grid, dim3(512), 0, st, a, slots);
     else hipLaunchKernelGGL((k_attn_rows<F16, 256, 4>), grid, dim3(256), 0, st, a, slots);
 }
@@ -1067,7 +1072,7 @@ using namespace wisp;
 
 extern "C" int64_t wisp_attn_prompt_ws_bytes(int64_t T, int B, int hq, int hk, int d, int page, int width) {
     if (T < 0 || B < 1 || hk < 1 || hq < hk || hq % hk || d < 64 || page < 1 || width < 1) return -1;
-    const int parts = row_parts(row_slots(T, B, hq / hk, rows_of(d)) * hk, (int64_t)page * width);
+    const int parts = row_parts(row_slots(T, B, hq / hk, rows_of(d, T * (hq / hk), hk)) * hk, (int64_t)page * width);
     return parts > 1 ? rec_bytes(T * hq * parts, d) : 0;
 }
 
@@ -1082,7 +1087,7 @@ extern "C" int wisp_attn_prompt(const void* q, int64_t q_ts, int64_t q_hs, const
     if (T == 0) return WISP_OK;
     if (!q || !cu || !kv_len || !table || !out) return fail_inval("null pointer");
     if (int rc = check_q(q, q_ts, q_hs, out)) return rc;
-    const int bm = rows_of(d);
+    const int bm = rows_of(d, T * (hq / hk), hk);
     const int64_t slots = row_slots(T, B, hq / hk, bm);
     const int parts = row_parts(slots * hk, (int64_t)page * width);
     if (parts > 1 && !ws) return fail_inval("null workspace");
@@ -1091,8 +1096,8 @@ extern "C" int wisp_attn_prompt(const void* q, int64_t q_ts, int64_t q_hs, const
     RowsArgs a{(const uint16_t*)q, q_ts, q_hs, paged_kv((void*)kc, (void*)vc, pages, page, page_stride, head_stride, row_stride),
                cu, kv_len, table, width, B, (int)T, hq, hk, hq / hk, 1.f / (float)(hq / hk), scale * 1.44269504088896340736f, parts, kPartTiles, ml, po, (uint16_t*)out};
     hipStream_t st = (hipStream_t)stream;
-    if (dtype == WISP_DT_F16) launch_rows<true>(a, d, (int)slots, st);
-    else launch_rows<false>(a, d, (int)slots, st);
+    if (dtype == WISP_DT_F16) launch_rows<true>(a, d, bm, (int)slots, st);
+    else launch_rows<false>(a, d, bm, (int)slots, st);
     if (parts > 1) {
         JoinArgs j{nullptr, nullptr, nullptr, nullptr, cu, kv_len, ml, po, parts, kPartTiles, bm, B, (int)T, hq, hk, width * page, 0, a.c, (uint16_t*)out};
         if (dtype == WISP_DT_F16) launch_join<true>(j, d, (unsigned)(T * hq), st);
@@ -1103,7 +1108,7 @@ extern "C" int wisp_attn_prompt(const void* q, int64_t q_ts, int64_t q_hs, const
 
 // The parts of a shared prefix: rows of all B sequences together.
 static int prefix_parts(int B, int hq, int hk, int d, int64_t positions) {
-    const int bm = rows_of(d);
+    const int bm = rows_of(d, (int64_t)B * (hq / hk), hk);
     const int n = row_parts((int64_t)(((int64_t)B * (hq / hk) + bm - 1) / bm) * hk, positions);
     return n < kMaxParts ? n : kMaxParts;
 }
@@ -1146,13 +1151,13 @@ extern "C" int wisp_attn_batch(const void* q, int64_t q_ts, int64_t q_hs, const 
     if (prefix_width && !f.single) f.out = nullptr;
     JoinArgs j{f.first, kv_len, f.ml, f.po, nullptr, nullptr, nullptr, nullptr, 0, 1, 1, B, B, hq, hk, 0, 0, c, (uint16_t*)out};
     if (prefix_width) {
-        const int bm = rows_of(d), slots = (int)(((int64_t)B * (hq / hk) + bm - 1) / bm);
+        const int bm = rows_of(d, (int64_t)B * (hq / hk), hk), slots = (int)(((int64_t)B * (hq / hk) + bm - 1) / bm);
         const int parts = prefix_parts(B, hq, hk, d, (int64_t)page * prefix_width);
         float* rml = (float*)(p + w.end);
         RowsArgs a{(const uint16_t*)q, q_ts, q_hs, kv, nullptr, prefix_len, prefix_table, prefix_width, B, B, hq, hk, hq / hk, 1.f / (float)(hq / hk), c, parts, 1,
                    rml, rml + 2 * (int64_t)B * hq * parts, nullptr};
-        if (f16) launch_rows<true>(a, d, slots, st);
-        else launch_rows<false>(a, d, slots, st);
+        if (f16) launch_rows<true>(a, d, bm, slots, st);
+        else launch_rows<false>(a, d, bm, slots, st);
         j.rml = f.rml = a.ml;
         j.rpo = f.rpo = a.po;
         j.nsplit = f.nsplit = parts;
