@@ -11,7 +11,10 @@
 //
 // HBM-bound: each element is read once and written once. A lane holds 16 bytes (8 elements) of a head, so D/8 lanes
 // share a head and a wave takes 512/D heads at a time; the sum of squares and the partner's values move between those
-// lanes. A wave walks some of its token's head groups with the token's cos and sin in registers.
+// lanes by DPP. A wave walks its token's head groups, the next group's load ahead of this one's stores. What hides the
+// latencies is the number of waves: cos, sin and the norm weights stay packed, so that the kernel fits 64 registers and
+// 8 waves a SIMD (with 85: 43 us for 6,976 tokens of 40 heads of 128, where 61 take 34.6 and, a wave a token, 31.3:
+// 4.7 TB/s).
 #include "paged.hpp"
 #include "wisp_device.hpp"
 #include "wisp_internal.hpp"
@@ -27,7 +30,7 @@ struct AppendArgs {
     int64_t cs_rows;
     int rot;
     const int *cu, *kv_len, *table;
-    int width, B, T, hq, hk, per_wave;  // per_wave: head groups a wave takes
+    int width, B, T, hq, hk, per_wave, waves;  // head groups a wave takes, waves of a token
     PagedKV kv;
     uint16_t* qo;  // [T][hq][D]
 };
@@ -51,51 +54,90 @@ __device__ __forceinline__ uint32_t round2(float lo, float hi) {
     }
 }
 
-template <bool F16, int D, bool INTER, bool CS32>
+// Sum over the lanes of a head (D/8 of them, consecutive), in every one of them.
+template <int D>
+__device__ __forceinline__ float head_sum(float v) {
+    v += dpp_f<0xB1>(v);   // xor 1
+    v += dpp_f<0x4E>(v);   // xor 2
+    v += dpp_f<0x141>(v);  // row_half_mirror: the other four of eight
+    if constexpr (D >= 128) v += dpp_f<0x140>(v);  // row_mirror: the other eight of a row
+    if constexpr (D == 256) v = add_xor16(v);
+    return v;
+}
+// The value of the lane that holds the other half of the head's pairs, rot/2 elements away (the whole head rotated).
+template <int D>
+__device__ __forceinline__ uint32_t other_half(uint32_t v) {
+    if constexpr (D == 64) {  // xor 4: row_half_mirror, then each quad reversed
+        const int m = __builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xF, 0xF, true);
+        return (uint32_t)__builtin_amdgcn_update_dpp(0, m, 0x1B, 0xF, 0xF, true);
+    } else if constexpr (D == 128) {  // xor 8: row_ror:8
+        return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xF, 0xF, true);
+    } else {  // xor 16: the swap leaves the partner's value in one of its two results
+        const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        return (threadIdx.x & 16) ? r[0] : r[1];
+    }
+}
+
+// ROT: 0 half pairs of a part of the head, 1 half pairs of the whole head, 2 interleaved
+template <bool F16, int D, int ROT, bool CS32>
 __global__ __launch_bounds__(256) void k_kv_append(const AppendArgs a) {
+    constexpr bool INTER = ROT == 2;
     constexpr int LPH = D / 8, HPW = 64 / LPH;  // lanes per head, heads per wave
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int hl = lane & (LPH - 1), hw = lane / LPH, e0 = 8 * hl;
     const int heads = a.hq + 2 * a.hk, groups = (heads + HPW - 1) / HPW;
-    const int waves = (groups + a.per_wave - 1) / a.per_wave;  // per token
-    const int64_t id = (int64_t)blockIdx.x * 4 + wv;
-    const int tok = (int)(id / waves), g0 = (int)(id - (int64_t)tok * waves) * a.per_wave;
+    const uint32_t id = blockIdx.x * 4u + wv;
+    const int tok = (int)(id / (uint32_t)a.waves), g0 = (int)(id - (uint32_t)tok * a.waves) * a.per_wave;
     if (tok >= a.T) return;
 
-    // the token's sequence: the last b whose range begins at or before it
-    int lo = 0, hi = a.B;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (a.cu[mid] <= tok) lo = mid;
-        else hi = mid;
-    }
-    int t0, t1;
-    token_range(a.cu, lo, a.T, t0, t1);
-    if (tok < t0 || tok >= t1) return;  // a row that belongs to no sequence
-    const int pos = a.kv_len[lo] - (t1 - tok);
-    bool bad = pos < 0 || pos >= a.cs_rows;
-    const int64_t at = page_offset(a.kv, a.table + (int64_t)lo * a.width, a.width, bad ? 0 : pos, bad);
+    auto load = [&](int g) {
+        const int h = min(g * HPW + hw, heads - 1);
+        const uint16_t* x = h < a.hq          ? a.q + tok * a.q_ts + h * a.q_hs
+                            : h < a.hq + a.hk ? a.k + tok * a.k_ts + (h - a.hq) * a.k_hs
+                                              : a.v + tok * a.v_ts + (h - a.hq - a.hk) * a.v_hs;
+        return *reinterpret_cast<const uint4*>(x + e0);
+    };
+    uint4 next = load(g0);
 
-    const bool rotated = e0 < a.rot;  // rot is a multiple of 16: a lane's eight elements are rotated or not together
+    // the token's sequence: the one whose range ends past it first; 64 ends are looked at together
+    int b = 0, t1 = 0, len = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 64) {
+        const int i = min(b0 + lane, a.B - 1), e = a.cu[i + 1], n = a.kv_len[i];
+        const uint64_t past = __ballot(b0 + lane < a.B && e > tok);
+        if (past) {
+            const int w = __builtin_ctzll(past);
+            b = b0 + w;
+            t1 = min(__builtin_amdgcn_readlane(e, w), a.T);
+            len = __builtin_amdgcn_readlane(n, w);
+            break;
+        }
+    }
+    if (t1 == 0 || scalar_at(a.cu, 0) > tok) return;  // a row that belongs to no sequence
+    const int pos = len - (t1 - tok);
+    bool bad = pos < 0 || pos >= a.cs_rows;
+    const int64_t at = page_offset(a.kv, a.table + (int64_t)b * a.width, a.width, bad ? 0 : pos, bad);
+
+    const bool rotated = ROT == 1 || e0 < a.rot;  // rot is a multiple of 16: a lane's eight elements are rotated or not together
     const int half = a.rot >> 1;
     const bool first = e0 < half;
     const int partner = rotated && !INTER ? (first ? hl + half / 8 : hl - half / 8) : hl;
-    float cs[8], sn[8];
+    // the lane's cos and sin, as they are stored (pairs of the type, or binary32)
+    constexpr int CN = CS32 ? 2 : 1;
+    uint4 cs[CN], sn[CN];
     {
         const int64_t r = bad ? 0 : (int64_t)pos * a.rot + (rotated ? e0 : 0);
-        if constexpr (CS32) {
-            const float *c = (const float*)a.cos + r, *s = (const float*)a.sin + r;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) cs[i] = c[i], sn[i] = s[i];
-        } else {
-            widen8<F16>(*reinterpret_cast<const uint4*>((const uint16_t*)a.cos + r), cs);
-            widen8<F16>(*reinterpret_cast<const uint4*>((const uint16_t*)a.sin + r), sn);
+        for (int i = 0; i < CN; ++i) {
+            cs[i] = *(reinterpret_cast<const uint4*>((const uint8_t*)a.cos + r * (CS32 ? 4 : 2)) + i);
+            sn[i] = *(reinterpret_cast<const uint4*>((const uint8_t*)a.sin + r * (CS32 ? 4 : 2)) + i);
         }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if (INTER ? (i & 1) == 0 : first) sn[i] = -sn[i];
-            if (!rotated) cs[i] = 1.f, sn[i] = 0.f;
-        }
+    }
+    const float sign = first ? -1.f : 1.f;  // of the partner's term
+    const bool norm = a.qw != nullptr;
+    uint4 w[2] = {};  // the lane's norm weights, of q and of k
+    if (norm) {
+        w[0] = *reinterpret_cast<const uint4*>(a.qw + e0);
+        w[1] = *reinterpret_cast<const uint4*>(a.kw + e0);
     }
     const float nan = __int_as_float(0x7FC00000);
     const int g1 = min(g0 + a.per_wave, groups);
@@ -103,53 +145,48 @@ __global__ __launch_bounds__(256) void k_kv_append(const AppendArgs a) {
         const int h = g * HPW + hw;
         const bool is_q = h < a.hq, is_k = !is_q && h < a.hq + a.hk;
         const bool have = h < heads;
-        uint4 raw = make_uint4(0, 0, 0, 0);
-        if (have) {
-            const uint16_t* x = is_q   ? a.q + tok * a.q_ts + h * a.q_hs
-                                : is_k ? a.k + tok * a.k_ts + (h - a.hq) * a.k_hs
-                                       : a.v + tok * a.v_ts + (h - a.hq - a.hk) * a.v_hs;
-            raw = *reinterpret_cast<const uint4*>(x + e0);
-        }
-        uint4 res = raw;
-        float x[8], xp[8];
-        widen8<F16>(raw, x);
-        float rs = 1.f;
-        if (a.qw) {
-            float ss = 0.f;
+        uint4 res = next;
+        if (g + 1 < g1) next = load(g + 1);  // ahead of this group's stores
+        if (g * HPW < a.hq + a.hk) {  // (values are copied)
+            float x[8];
+            widen8<F16>(res, x);
+            if (norm) {
+                float ss = 0.f, f[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(x[i], x[i], ss);
+                for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(x[i], x[i], ss);
+                const float rs = rsqrtf(head_sum<D>(ss) * (1.f / D) + a.eps);
+                widen8<F16>(is_q ? w[0] : w[1], f);
 #pragma unroll
-            for (int o = 1; o < LPH; o <<= 1) ss += __shfl_xor(ss, o, 64);
-            rs = rsqrtf(ss * (1.f / D) + a.eps);
-        }
-        uint4 other = raw;
-        if constexpr (!INTER) {
-            const int src = hw * LPH + partner;
-            other.x = __shfl((int)raw.x, src, 64);
-            other.y = __shfl((int)raw.y, src, 64);
-            other.z = __shfl((int)raw.z, src, 64);
-            other.w = __shfl((int)raw.w, src, 64);
-        }
-        widen8<F16>(other, xp);
-        if (is_q || is_k) {
-            if (a.qw) {
-                const uint16_t* w = is_q ? a.qw : a.kw;
-                float wv8[8], wp[8];
-                widen8<F16>(*reinterpret_cast<const uint4*>(w + e0), wv8);
-                widen8<F16>(*reinterpret_cast<const uint4*>(w + 8 * partner), wp);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = x[i] * rs * wv8[i], xp[i] = xp[i] * rs * wp[i];
+                for (int i = 0; i < 8; ++i) x[i] = x[i] * rs * f[i];
             }
             float y[8];
+            float c[8], sv[8];
+            if constexpr (CS32) {
+                const uint32_t cw[8] = {cs[0].x, cs[0].y, cs[0].z, cs[0].w, cs[1].x, cs[1].y, cs[1].z, cs[1].w};
+                const uint32_t sw[8] = {sn[0].x, sn[0].y, sn[0].z, sn[0].w, sn[1].x, sn[1].y, sn[1].z, sn[1].w};
+#pragma unroll
+                for (int i = 0; i < 8; ++i) c[i] = __uint_as_float(cw[i]), sv[i] = __uint_as_float(sw[i]);
+            } else {
+                widen8<F16>(cs[0], c);
+                widen8<F16>(sn[0], sv);
+            }
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
+                float t;
+                if constexpr (INTER) t = i & 1 ? x[i ^ 1] : -x[i ^ 1];
+                else if constexpr (ROT == 1) t = sign * __uint_as_float(other_half<D>(__float_as_uint(x[i])));
+                else t = sign * __shfl(x[i], hw * LPH + partner, 64);
                 // unrotated elements: y = x exactly, whatever the partner holds
-                const float t = INTER ? x[i ^ 1] : xp[i];
-                y[i] = rotated ? __builtin_fmaf(x[i], cs[i], t * sn[i]) : x[i];
-                if (bad) y[i] = nan;
+                y[i] = rotated ? __builtin_fmaf(x[i], c[i], t * sv[i]) : x[i];
             }
-            res = make_uint4(round2<F16>(y[0], y[1]), round2<F16>(y[2], y[3]), round2<F16>(y[4], y[5]),
-                             round2<F16>(y[6], y[7]));
+            if (is_q || is_k) {
+                res = make_uint4(round2<F16>(y[0], y[1]), round2<F16>(y[2], y[3]), round2<F16>(y[4], y[5]),
+                                 round2<F16>(y[6], y[7]));
+                if (bad) {
+                    const uint32_t n2 = round2<F16>(nan, nan);
+                    res = make_uint4(n2, n2, n2, n2);
+                }
+            }
         }
         if (is_q) {
             *reinterpret_cast<uint4*>(a.qo + ((int64_t)tok * a.hq + h) * D + e0) = res;
@@ -161,13 +198,15 @@ __global__ __launch_bounds__(256) void k_kv_append(const AppendArgs a) {
 }
 
 template <bool F16, int D>
-static void launch_append(const AppendArgs& a, bool inter, bool cs32, dim3 grid, hipStream_t st) {
-#define WISP_APPEND(I, C) \
-    if (inter == I && cs32 == C) hipLaunchKernelGGL((k_kv_append<F16, D, I, C>), grid, dim3(256), 0, st, a);
-    WISP_APPEND(false, false)
-    WISP_APPEND(false, true)
-    WISP_APPEND(true, false)
-    WISP_APPEND(true, true)
+static void launch_append(const AppendArgs& a, int rot, bool cs32, dim3 grid, hipStream_t st) {
+#define WISP_APPEND(R, C) \
+    if (rot == R && cs32 == C) hipLaunchKernelGGL((k_kv_append<F16, D, R, C>), grid, dim3(256), 0, st, a);
+    WISP_APPEND(0, false)
+    WISP_APPEND(0, true)
+    WISP_APPEND(1, false)
+    WISP_APPEND(1, true)
+    WISP_APPEND(2, false)
+    WISP_APPEND(2, true)
 #undef WISP_APPEND
 }
 
@@ -202,20 +241,24 @@ extern "C" int wisp_kv_append(const void* q, int64_t q_ts, int64_t q_hs, const v
             return WISP_EALIGN;
         }
     const int hpw = 512 / d, groups = (hq + 2 * hk + hpw - 1) / hpw;
-    // Few tokens: a wave per head group, so that the call has as many requests in flight as it can; many: a wave walks
-    // more of its token's groups and loads cos, sin and the page id less often.
+    // Few tokens: a wave per head group, so that the call has as many requests in flight as it can. Enough for a wave each
+    // to fill most of the 8,192 that the card holds: a wave walks all its token's groups and finds cos, sin and the page
+    // once (6,976 tokens of 40 heads: 34.6 -> 31.3 us). Between them, two to three times the card's waves (4,153 tokens of
+    // 20 heads of 256: 23.1 us; 24.3 with one wave a token, 25.4 with two, just past a full round).
     int per_wave = 1;
+    if (T >= 6144) per_wave = groups;
     while (per_wave < groups && T * ((groups + 2 * per_wave - 1) / (2 * per_wave)) >= 16384) per_wave *= 2;
     const int waves = (groups + per_wave - 1) / per_wave;
     AppendArgs a{(const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, q_ts, q_hs, k_ts, k_hs, v_ts, v_hs,
                  (const uint16_t*)q_norm_w, (const uint16_t*)k_norm_w, eps, cos, sin, cs_rows, rot, cu, kv_len, table,
-                 width, B, (int)T, hq, hk, per_wave, paged_kv(kc, vc, pages, page, page_stride, head_stride, row_stride),
+                 width, B, (int)T, hq, hk, per_wave, waves, paged_kv(kc, vc, pages, page, page_stride, head_stride, row_stride),
                  (uint16_t*)qo};
     const int64_t blocks = (T * waves + 3) / 4;
-    if (blocks > 0x7FFFFFFF) return fail_inval("too many tokens for one call");
+    if (blocks > 0x3FFFFFFF) return fail_inval("too many tokens for one call");
     const dim3 grid((unsigned)blocks);
     hipStream_t st = (hipStream_t)stream;
-    const bool cs32 = cs_dtype == WISP_DT_F32, in = interleaved != 0;
+    const bool cs32 = cs_dtype == WISP_DT_F32;
+    const int in = interleaved ? 2 : rot == d ? 1 : 0;
     if (dtype == WISP_DT_F16) {
         if (d == 64) launch_append<true, 64>(a, in, cs32, grid, st);
         else if (d == 128) launch_append<true, 128>(a, in, cs32, grid, st);
