@@ -87,7 +87,7 @@ __device__ __forceinline__ uint2 read_tr(const uint8_t* p) {
 __device__ __forceinline__ uint32_t lds_addr(const void* p) { return (uint32_t)(uintptr_t)p; }
 // 64 lanes x 16 bytes from base + each lane's 32-bit offset to LDS [lds, lds + 1024). The compiler neither emits nor counts
 // these loads: the waits for them are wait_vm<n>, n = the loads issued after the awaited ones. M0 is written here only
-// (a reserved register: the clobber is advisory), which tests/test_paged_isa.py checks.
+// (a reserved register: the clobber is advisory), which tests/test_paged.py checks.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void dma16(uint32_t lds, const uint8_t* base, uint32_t off) {
@@ -258,47 +258,43 @@ __global__ __launch_bounds__(64 * NW, D == 64 && NW == 4 ? 3 : 1) void k_attn_ro
     const int tiles = (t.end + kTile - 1) / kTile;
     const int parts = a.out ? parts_of(tiles, a.nsplit, a.part_min) : a.nsplit;
     if (part >= parts) return;
-    // (tiles <= 2^24, parts <= 256)
-    const int j0 = parts > 1 ? (uint32_t)tiles * part / parts : 0, j1 = parts > 1 ? (uint32_t)tiles * (part + 1) / parts : tiles;
+    const int j0 = parts > 1 ? (int)((uint64_t)tiles * part / parts) : 0, j1 = parts > 1 ? (int)((uint64_t)tiles * (part + 1) / parts) : tiles;
     if (threadIdx.x == 0) bad_l = odd_l = 0;
 
     const int* trow = a.table + (int64_t)t.b * a.width;
     const uint8_t* kbase = a.kv.kc + head * a.kv.hs;
     const uint8_t* vbase = a.kv.vc + head * a.kv.hs;
-    // instruction i of this wave fills rows RPI (wv + NW i) .. of the tile; lane: row lane / (RB/16), stored chunk
-    // lane % (RB/16)
-    constexpr int SAME = RPI * NW % 16 == 0 ? 1 : LPW;  // the permutation has period 16 in the row
+    // instruction i of this wave fills rows PW wv + RPI i .. of the tile, all of one page; lane: row lane / (RB/16), stored
+    // chunk lane % (RB/16)
+    constexpr int PW = kTile / NW;
     const int dr = lane / (RB / 16), dc = lane % (RB / 16);
-    uint32_t ko[SAME], vo[SAME];
+    uint32_t ko[LPW], vo[LPW];
 #pragma unroll
-    for (int i = 0; i < SAME; ++i) {
-        const int r = RPI * (wv + NW * i) + dr;
+    for (int i = 0; i < LPW; ++i) {
+        const int r = PW * wv + RPI * i + dr;
         ko[i] = (uint32_t)(dr * (int)a.kv.rs + 16 * swz_k<D>(r, dc));
         vo[i] = (uint32_t)(dr * (int)a.kv.rs + 16 * swz_v<D, false>(r, dc));
     }
     bool bad = t.bad;
     const int last_row = max(0, t.end - 1) & ~(RPI - 1);
-    // Tile j's page ids, read a turn before its loads are issued (rows past the end repeat the last ones: their page exists).
-    int page[LPW];
-    auto row_of = [&](int j, int i) { return min(j * kTile + RPI * (wv + NW * i), last_row); };
+    // Tile j's page id, read a turn before its loads are issued (rows past the end repeat the last ones: their page exists).
+    int page;
     auto find_pages = [&](int j) {
-#pragma unroll
-        for (int i = 0; i < LPW; ++i) {
-            const int at = row_of(j, i) >> a.kv.shift;
-            page[i] = scalar_at(trow, min(at, a.width - 1));
-            if (at >= a.width) page[i] = -1;
-        }
+        const int at = min(j * kTile + PW * wv, last_row) >> a.kv.shift;
+        page = scalar_at(trow, min(at, a.width - 1));
+        if (at >= a.width) page = -1;
     };
     auto issue = [&](int j) {
-        const uint32_t st = lds_addr(&buf[j & (NST - 1)][0][0]);
+        const uint32_t st = lds_addr(&buf[j & (NST - 1)][0][0]) + PW * wv * RB;
+        const bool ok = (unsigned)page < (unsigned)a.kv.pages;
+        bad = bad || !ok;
+        const int64_t off = (ok ? (int64_t)page : 0) * a.kv.ps;
 #pragma unroll
         for (int i = 0; i < LPW; ++i) {
-            const int r = RPI * (wv + NW * i);
-            const bool ok = (unsigned)page[i] < (unsigned)a.kv.pages;
-            bad = bad || !ok;
-            const int64_t off = (ok ? (int64_t)page[i] : 0) * a.kv.ps + (int64_t)(row_of(j, i) & ((1 << a.kv.shift) - 1)) * a.kv.rs;
-            dma16(st + r * RB, uniform(kbase + off), ko[i % SAME]);
-            dma16(st + TB + r * RB, uniform(vbase + off), vo[i % SAME]);
+            const int row = min(j * kTile + PW * wv + RPI * i, last_row) & ((1 << a.kv.shift) - 1);
+            const int64_t at = off + (int64_t)row * a.kv.rs;
+            dma16(st + i * 1024, uniform(kbase + at), ko[i]);
+            dma16(st + TB + i * 1024, uniform(vbase + at), vo[i]);
         }
     };
     const bool late = TURNS && wv >= NW / 2;
@@ -515,8 +511,10 @@ __global__ __launch_bounds__(64 * NW, D == 64 && NW == 4 ? 3 : 1) void k_attn_ro
             }
             if (active && lim_hi >= j * kTile) {
                 scores(j);
+                if constexpr (D == 256) order_turn<0, 2 * KD>();  // (one wave a SIMD: 132 us, 155 without, at 3,000 tokens)
                 weigh(j);
                 collect(j);
+                if constexpr (D == 256) order_turn<4 * ND, 0>();
             }
         }
     }
@@ -989,7 +987,9 @@ __global__ __launch_bounds__(256) void k_attn_join(const JoinArgs a) {
 }
 
 // ---------------------------------------------------------------------------
-// Query rows of a k_attn_rows workgroup. D = 256: four waves, whose registers the CU's whole file holds. D = 128: eight.
+// Query rows of a k_attn_rows workgroup. D = 256: four waves, whose registers the CU's whole file holds (16 query and 2 K/V
+// heads, 3,000 tokens: 113 us; eight waves with tiles of 32 positions 207, 16 over 8 heads and 8,000 tokens 598 and 582).
+// D = 128: eight.
 // D = 64, where a tile's weights cost twice its matrix products: four waves, four workgroups to a CU,
 // where there are enough to keep them all busy (64 query and 8 K/V heads, 4,000 tokens: 164 -> 150 us; 1,500 in three
 // prompts: 28.4 -> 26.3), else eight waves that take turns (1,018 tokens behind 24,000: 399 us, 428 with four).
