@@ -633,3 +633,100 @@ def test_another_stream_and_repeated_calls():
     torch.cuda.synchronize()
     for a, b in got:
         assert torch.equal(a, want) and torch.equal(b, want_p)
+
+
+def _heads(seed, T, hq, hk, D, dtype):
+    g = _gen(seed)
+    x = _rand(g, T, hq + 2 * hk, D, dtype=dtype)
+    return x[:, :hq], x[:, hq : hq + hk], x[:, hq + hk :]
+
+
+@pytest.mark.parametrize("dtype,D,inter", [(BF, 128, False), (HF, 64, True)])
+def test_append_of_many_tokens_is_that_of_its_slices(dtype, D, inter):
+    """However a call's heads are dealt out to waves, which follows its number of tokens, a token's result is the same."""
+    T, hq, hk = 6300, 32, 4
+    g = _gen(40)
+    table, P = _tables(g, [T], 64)
+    q, k, v = _heads(41, T, hq, hk, D, dtype)
+    cos, sin = _rope(g, T, D, dtype, inter, True)
+    w = [_rand(g, D, dtype=dtype) for _ in range(2)]
+    caches = [_cache(_gen(42), P, hk, 64, D, dtype) for _ in range(2)]
+    whole = kernels.kv_append(q, k, v, cos, sin, _i32([0, T]), _i32([T]), table, *caches[0], *w, interleaved=inter)
+    parts = []
+    for lo, hi in [(0, 1), (1, 700), (700, 4900), (4900, T)]:
+        parts.append(kernels.kv_append(q[lo:hi], k[lo:hi], v[lo:hi], cos, sin, _i32([0, hi - lo]), _i32([hi]), table, *caches[1],
+                                       *w, interleaved=inter))
+    assert torch.equal(whole, torch.cat(parts))
+    for a, b in zip(*caches):
+        assert torch.equal(a, b)
+
+
+def test_more_sequences_than_lanes():
+    new = [(5 * i) % 4 for i in range(150)]
+    ctx = [(29 * i) % 90 for i in range(150)]
+    s = _prompt(43, BF, 8, 2, 128, 16, new, ctx)
+    ref, A = _prompt_ref(s, new, ctx)
+    _check(kernels.attn_prompt(**s), ref, A, BF, False)
+    T = sum(new)
+    q, k, v = _heads(44, T, 8, 2, 128, BF)
+    cos, sin = _rope(_gen(45), 128, 128, BF, False, False)
+    caches = [[t.clone() for t in (s["kc"], s["vc"])] for _ in range(2)]
+    whole = kernels.kv_append(q, k, v, cos, sin, s["cu"], s["kv_len"], s["table"], *caches[0])
+    parts, cu = [], s["cu"].tolist()
+    for b in range(0, 150, 50):
+        lo, hi = cu[b], cu[b + 50]
+        parts.append(kernels.kv_append(q[lo:hi], k[lo:hi], v[lo:hi], cos, sin, s["cu"][b : b + 51] - lo, s["kv_len"][b : b + 50],
+                                       s["table"][b : b + 50], *caches[1]))
+    assert torch.equal(whole, torch.cat(parts))
+    for a, b in zip(*caches):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("D,hq,hk", [(64, 20, 1), (128, 32, 4), (256, 8, 8)])
+def test_results_over_their_queries(D, hq, hk):
+    for new, ctx in [([70, 3], [200, 900]), ([1], [6000])]:
+        p = _prompt(46, BF, hq, hk, D, 64, new, ctx)
+        want = kernels.attn_prompt(**p)
+        assert torch.equal(kernels.attn_prompt(**p, out=p["q"]), want) and torch.equal(p["q"], want)
+    for prefix in (None, 700):
+        for lens in ([300, 0, 40], [3000, 5]):
+            s = _batch(47, BF, hq, hk, D, 64, lens, prefix=prefix)
+            call = kernels.attn_shared if prefix else kernels.attn_batch
+            want = call(**s)
+            assert torch.equal(call(**s, out=s["q"]), want) and torch.equal(s["q"], want)
+    g = _gen(48)
+    q, k, v = (_rand(g, 40, h, D) for h in (hq, hk, hk))
+    cos, sin = _rope(g, 40, D, BF, False, True)
+    caches = [_cache(_gen(49), 1, hk, 64, D, BF) for _ in range(2)]
+    args = [cos, sin, _i32([0, 40]), _i32([40]), _i32([[0]])]
+    want = kernels.kv_append(q, k, v, *args, *caches[0])
+    assert torch.equal(kernels.kv_append(q, k, v, *args, *caches[1], qo=q), want)
+
+
+def test_the_same_pages_in_several_sequences():
+    s = _batch(50, BF, 32, 4, 128, 64, [700, 700, 130])
+    s["table"][1:] = s["table"][0]
+    ref, A = _batch_ref(s, [700, 700, 130])
+    _check(kernels.attn_batch(**s), ref, A, BF, True)
+    p = _prompt(51, HF, 8, 2, 64, 32, [9, 40], [300, 64])
+    p["table"][1] = p["table"][0]
+    ref, A = _prompt_ref(p, [9, 40], [300, 64])
+    _check(kernels.attn_prompt(**p), ref, A, HF, False)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_a_query_that_is_not_finite_spoils_its_own_row_only(D):
+    p = _prompt(52, BF, 8, 2, D, 64, [50], [170])
+    ref, A = _prompt_ref(p, [50], [170])
+    p["q"][17, 3, 5] = math.nan
+    got = kernels.attn_prompt(**p)
+    assert got[17, 3].isnan().all()
+    got[17, 3], ref[17, 3] = 0, 0
+    _check(got, ref, A, BF, False)
+    s = _batch(53, BF, 8, 2, D, 64, [50, 900])
+    ref, A = _batch_ref(s, [50, 900])
+    s["q"][1, 6, 0] = math.nan
+    got = kernels.attn_batch(**s)
+    assert got[1, 6].isnan().all()
+    got[1, 6], ref[1, 6] = 0, 0
+    _check(got, ref, A, BF, True)
