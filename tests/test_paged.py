@@ -164,3 +164,11 @@ def test_m0_is_written_by_the_direct_loads_only():
         elif re.search(r"\bm0\b", s.split(";", 1)[0]):
             other.append(s)
     assert dma > 0 and not other, other[:5]
+
+
+def test_token_counts_past_any_call_are_refused():
+    L = _lib.lib()
+    for T in (1 << 31, 1 << 62):
+        assert L.wisp_attn_prompt_ws_bytes(T, 1, 32, 4, 128, 64, 256) == -1
+        assert _prompt(T=T) == -1
+        assert _append(T=T) == -1

@@ -730,3 +730,17 @@ def test_a_query_that_is_not_finite_spoils_its_own_row_only(D):
     assert got[1, 6].isnan().all()
     got[1, 6], ref[1, 6] = 0, 0
     _check(got, ref, A, BF, True)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_rows_whose_scores_are_all_minus_infinity_give_zeros(D):
+    p = _prompt(54, BF, 8, 2, D, 64, [40], [100])
+    p["q"][..., 0] = 1
+    p["kc"][..., 0] = -math.inf
+    assert (kernels.attn_prompt(**p) == 0).all()
+    s = _batch(55, BF, 8, 2, D, 64, [40, 3000], prefix=300)
+    s["q"][..., 0] = 1
+    s["kc"][..., 0] = -math.inf
+    assert (kernels.attn_shared(**s) == 0).all()
+    del s["prefix_len"], s["prefix_table"]
+    assert (kernels.attn_batch(**s) == 0).all()

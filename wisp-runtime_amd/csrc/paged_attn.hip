@@ -1071,7 +1071,7 @@ int check_q(const void* q, int64_t q_ts, int64_t q_hs, const void* out) {
 using namespace wisp;
 
 extern "C" int64_t wisp_attn_prompt_ws_bytes(int64_t T, int B, int hq, int hk, int d, int page, int width) {
-    if (T < 0 || B < 1 || hk < 1 || hq < hk || hq % hk || d < 64 || page < 1 || width < 1) return -1;
+    if (T < 0 || T > (1 << 30) || B < 1 || hk < 1 || hq < hk || hq > 1024 || hq % hk || d < 64 || page < 1 || width < 1) return -1;
     const int parts = row_parts(row_slots(T, B, hq / hk, rows_of(d, T * (hq / hk), hk)) * hk, (int64_t)page * width);
     return parts > 1 ? rec_bytes(T * hq * parts, d) : 0;
 }
@@ -1082,7 +1082,7 @@ extern "C" int wisp_attn_prompt(const void* q, int64_t q_ts, int64_t q_hs, const
                                 int d, int dtype, float scale, void* ws, void* out, void* stream) {
     clear_error();
     if (int rc = check_paged(kc, vc, pages, page, page_stride, head_stride, row_stride, width, B, hq, hk, d, dtype)) return rc;
-    if (T < 0 || T * hq > (1 << 30)) return fail_inval("T * hq must be in [0, 2^30]");
+    if (T < 0 || T > (1 << 30) || T * hq > (1 << 30)) return fail_inval("T * hq must be in [0, 2^30]");
     if (!good_scale(scale)) return fail_inval("scale must be positive and finite");
     if (T == 0) return WISP_OK;
     if (!q || !cu || !kv_len || !table || !out) return fail_inval("null pointer");
