@@ -252,22 +252,13 @@ def _plain_attend(s):
     return out
 
 
-_kernels = None
-
-
-def _package():
-    """The package's kernels module, imported once, as a program does."""
-    global _kernels
-    if _kernels is None:
-        root = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "wisp-runtime_amd")
-        if root not in sys.path:
-            sys.path.insert(0, root)
-        from wisp import kernels as _kernels
-    return _kernels
-
-
 def _own(s):
-    kernels, kind = _package(), s["kind"]
+    root = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "wisp-runtime_amd")
+    if root not in sys.path:
+        sys.path.insert(0, root)
+    from wisp import kernels
+
+    kind = s["kind"]
     if kind == "append":
         q = kernels.kv_append(s["q"], s["k"], s["v"], s["cos"], s["sin"], s["cu"], s["kv_len"], s["table"], s["kc"], s["vc"],
                               q_norm_w=s["qn"], k_norm_w=s["kn"], eps=EPS, interleaved=s["inter"])
