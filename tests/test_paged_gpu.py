@@ -744,3 +744,59 @@ def test_rows_whose_scores_are_all_minus_infinity_give_zeros(D):
     assert (kernels.attn_shared(**s) == 0).all()
     del s["prefix_len"], s["prefix_table"]
     assert (kernels.attn_batch(**s) == 0).all()
+
+
+@pytest.mark.parametrize("dtype,hq,hk,D", [(BF, 32, 4, 128), (HF, 20, 1, 64), (BF, 6, 2, 64), (HF, 16, 2, 256), (BF, 3, 3, 256)])
+@pytest.mark.parametrize("lens,prefix", [([40, 3000, 700], None), ([300, 129, 0], None), ([40, 200, 700], 900), ([5, 1500, 33], 2100)])
+def test_an_infinite_value_that_is_attended_gives_an_infinity(dtype, hq, hk, D, lens, prefix):
+    """Weights are split in two terms, of which the second is often 0 or negative. Own positions and a prefix's, cut into pieces
+    or taken whole; every other element as it is without the infinity, bit for bit."""
+    call = kernels.attn_shared if prefix else kernels.attn_batch
+    s = _batch(60, dtype, hq, hk, D, 32, lens, "nhd", prefix=prefix)
+    want = call(**s)
+    rows = [("table", 0, 17 % lens[0], [0]), ("table", 1, lens[1] - 1, [1])]
+    if prefix:
+        rows.append(("prefix", None, 515, [0, 1, 2]))
+    for where, b, p, hit in rows:
+        page = int(s["prefix_table"][p // 32] if where == "prefix" else s["table"][b, p // 32])
+        for value in (math.inf, -math.inf, math.nan):
+            vc = s["vc"].clone()
+            vc[page, :, p % 32, 7] = value
+            vc[page, :, p % 32, D - 1] = -value
+            got = call(**dict(s, vc=vc))
+            for d, v in ((7, value), (D - 1, -value)):
+                x = got[hit][:, :, d]
+                assert (x.isnan() if math.isnan(v) else x == v).all(), (where, value, d)
+            rest = torch.ones_like(want, dtype=torch.bool)
+            for h in hit:
+                rest[h, :, 7] = rest[h, :, D - 1] = False
+            assert torch.equal(got[rest], want[rest])
+    vc = s["vc"].clone()  # both signs: NaN
+    page = int(s["table"][1, 0])
+    vc[page, :, 3, 7], vc[page, :, 5, 7] = math.inf, -math.inf
+    got = call(**dict(s, vc=vc))
+    assert got[1, :, 7].isnan().all() and torch.isfinite(got[1, :, :7].float()).all()
+
+
+@pytest.mark.parametrize("dtype,D", [(HF, 64), (HF, 128), (HF, 256), (BF, 128)])
+def test_an_infinite_value_of_a_small_weight_gives_an_infinity(dtype, D):
+    """A weight of e^-30: 0 in float16, not in binary32. It is met in tiles that all rows attend and in others, before and
+    after the large weights. One of e^-200 is 0 in binary32, too: there the result is only known not to be finite."""
+    n, page = 700, 64
+    kc, vc = torch.zeros(11, 1, page, D, dtype=dtype, device=DEV), _rand(_gen(61), 11, 1, page, D, dtype=dtype)
+    table = torch.arange(11, dtype=torch.int32, device=DEV)[None]
+    q = torch.zeros(n, 2, D, dtype=dtype, device=DEV)
+    q[..., 0] = 1
+    for p, gap in ((3, 30), (100, 30), (599, 30), (3, 200)):
+        k, v = kc.clone(), vc.clone()
+        k[p // page, 0, p % page, 0] = -gap
+        v[p // page, 0, p % page, 9] = -math.inf
+        a = kernels.attn_prompt(q, k, v, _i32([0, n]), _i32([n]), table, 1.0)
+        b = kernels.attn_batch(q[:1], k, v, _i32([n]), table, 1.0)
+        c = kernels.attn_shared(q[:1], k, v, _i32([60]), table[:, 10:].contiguous(), _i32([640]), table[0, :10].contiguous(), 1.0)
+        hit = [a[p + 1 :, :, 9], b[..., 9], c[..., 9]]
+        for x in hit:
+            assert ((x == -math.inf) if gap == 30 else ~torch.isfinite(x.float())).all(), (p, gap)
+        for x in (a, b, c):
+            assert torch.isfinite(x[..., :9].float()).all() and torch.isfinite(x[..., 10:].float()).all()
+        assert torch.isfinite(a[:p].float()).all()

@@ -141,6 +141,46 @@ __device__ __forceinline__ uint32_t finite2(uint32_t u) {
     return (n & 0x8000u ? 0u : u & 0xFFFFu) | (n >> 31 ? 0u : u & 0xFFFF0000u);
 }
 
+// What four stored values hold besides finite ones, added to a: an infinity or NaN as it is, 0 for a finite one.
+template <bool F16>
+__device__ __forceinline__ void add_odd(uint2 u, f4_t& a) {
+    a[0] += lo_of<F16>(u.x) - lo_of<F16>(finite2<F16>(u.x));
+    a[1] += hi_of<F16>(u.x) - hi_of<F16>(finite2<F16>(u.x));
+    a[2] += lo_of<F16>(u.y) - lo_of<F16>(finite2<F16>(u.y));
+    a[3] += hi_of<F16>(u.y) - hi_of<F16>(finite2<F16>(u.y));
+}
+// A sum over attended values that has come out NaN (its statistics l are not): a weight that the type, or its second term,
+// rounds to 0, or a negative second term, has met an infinite value. Then the sum is that of the values that are not finite.
+__device__ __forceinline__ bool spoiled(float l, f4_t o) {
+    const float z = (fabsf(o[0]) + fabsf(o[1])) + (fabsf(o[2]) + fabsf(o[3]));
+    return fabsf(l) < INFINITY && z != z;
+}
+// Those values of four dims, added up over n rows of V: the lane's dims are the 8 bytes at own of row(i), all lanes' are the
+// 16 VECS bytes at first. 64 rows are looked at together.
+template <bool F16, int VECS, typename Row>
+__device__ __forceinline__ f4_t odd_sum(int n, int lane, int first, int own, Row row) {
+    f4_t sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+    for (int i0 = 0; i0 < n; i0 += 64) {
+        const uint4* r = reinterpret_cast<const uint4*>(row(min(i0 + lane, n - 1)) + first);
+        uint32_t odd = 0;
+#pragma unroll
+        for (int v = 0; v < VECS; ++v)
+            odd |= nonfinite2<F16>(r[v].x) | nonfinite2<F16>(r[v].y) | nonfinite2<F16>(r[v].z) | nonfinite2<F16>(r[v].w);
+#pragma unroll 1
+        for (uint64_t m = __ballot(i0 + lane < n && odd); m; m &= m - 1) {
+            add_odd<F16>(*reinterpret_cast<const uint2*>(row(i0 + __builtin_ctzll(m)) + own), sum);
+            if (!__any(sum[0] == sum[0] || sum[1] == sum[1] || sum[2] == sum[2] || sum[3] == sum[3])) return sum;  // NaN all
+        }
+    }
+    return sum;
+}
+__device__ __forceinline__ void mend(float l, f4_t& o, f4_t odd) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (fabsf(l) < INFINITY && o[i] != o[i] && odd[i] != 0.f) o[i] = odd[i];
+}
+
 // The order of a turn's LDS reads and matrix instructions: NV operands of V (two reads each), then NK of K (one read), each
 // read kAhead instructions before its use. (Left to itself the compiler reads two at a time and waits for them.)
 constexpr int kAhead = 4;
@@ -525,9 +565,27 @@ __global__ __launch_bounds__(64 * NW, D == 64 && NW == 4 ? 3 : 1) void k_attn_ro
     if (bad) bad_l = 1;  // any wave's
     barrier();
     if (!active) return;
+    l = add_xor32(l);
+    const int p_odd = max(j0 * kTile, (lim_wg + 1) & ~(kTile - 1));  // the first tile with positions that not all rows attend
+    if constexpr (F16) {
+        // (bfloat16 weights have binary32's range; a float16 one below 2^-33 of the largest is 0.) The tiles up to p_odd:
+        const int n_even = min(p_odd, min(j1 * kTile, t.end)) - j0 * kTile;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                f4_t x = {o[d][4 * e], o[d][4 * e + 1], o[d][4 * e + 2], o[d][4 * e + 3]};
+                if (!__any(spoiled(l, x))) continue;
+                mend(l, x, odd_sum<F16, 1>(n_even, lane, 64 * d + 16 * e, 64 * d + 16 * e + 8 * hf, [&](int i) {
+                         return vbase + page_offset(a.kv, trow, a.width, j0 * kTile + i, bad);
+                     }));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[d][4 * e + i] = x[i];
+            }
+    }
     if (odd_l) {
 #pragma unroll 1
-        for (int p = max(j0 * kTile, (lim_wg + 1) & ~(kTile - 1)); p < min(j1 * kTile, t.end); ++p) {
+        for (int p = p_odd; p < min(j1 * kTile, t.end); ++p) {
             const uint8_t* vr = vbase + page_offset(a.kv, trow, a.width, p, bad) + 8 * hf;
 #pragma unroll
             for (int d = 0; d < ND; ++d)
@@ -535,15 +593,14 @@ __global__ __launch_bounds__(64 * NW, D == 64 && NW == 4 ? 3 : 1) void k_attn_ro
                 for (int e = 0; e < 4; ++e) {
                     const uint2 u = *reinterpret_cast<const uint2*>(vr + 64 * d + 16 * e);
                     if (p <= lim && (nonfinite2<F16>(u.x) | nonfinite2<F16>(u.y))) {
-                        o[d][4 * e] += lo_of<F16>(u.x) - lo_of<F16>(finite2<F16>(u.x));
-                        o[d][4 * e + 1] += hi_of<F16>(u.x) - hi_of<F16>(finite2<F16>(u.x));
-                        o[d][4 * e + 2] += lo_of<F16>(u.y) - lo_of<F16>(finite2<F16>(u.y));
-                        o[d][4 * e + 3] += hi_of<F16>(u.y) - hi_of<F16>(finite2<F16>(u.y));
+                        f4_t odd = {0.f, 0.f, 0.f, 0.f};
+                        add_odd<F16>(u, odd);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) o[d][4 * e + i] += odd[i];
                     }
                 }
         }
     }
-    l = add_xor32(l);
     const bool poison = bad_l != 0;
     // A lane's values lie in four-value runs of one row: through LDS, in the wave's own part of it (16-byte chunks permuted
     // as K's), to stores of whole rows.
@@ -807,6 +864,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_flat(const FlatA
     // the four waves' sums: o[d][i] = O[row n][dim 16 d + 4 r + i]
     l = add_xor32(add_xor16(l));
     if (bad) l = __int_as_float(0x7FC00000);
+    const int mine = max(0, to - p_first), n_mine = mine / kStep * kSub + min(mine % kStep, kSub);  // the wave's positions
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+        if (__any(spoiled(l, o[d])))
+            mend(l, o[d], odd_sum<F16, 2>(n_mine, lane, 32 * d, 32 * d + 8 * r, [&](int i) {
+                     return vbase + page_offset(a.kv, trow, a.width, p_first + i / kSub * kStep + i % kSub, bad);
+                 }));
     if (r == 0) {
         red[wv][n][0] = m;
         red[wv][n][1] = l;
@@ -835,6 +899,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_flat(const FlatA
 #pragma unroll
         for (int w = 0; w < 4; ++w) L += red[w][row][0] == -INFINITY ? red[w][row][1] : red[w][row][1] * __builtin_amdgcn_exp2f((red[w][row][0] - Mr) * c);
         float m[kMaxParts / 16], ll[kMaxParts / 16], Mx = Mr;
+        bool none[kMaxParts / 16];  // a record without weights
 #pragma unroll
         for (int k = 0; k < kMaxParts / 16; ++k) {
             const int p = e + 16 * k;
@@ -847,8 +912,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_flat(const FlatA
         float sum = 0.f;
 #pragma unroll
         for (int k = 0; k < kMaxParts / 16; ++k) {
-            const float w = m[k] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m[k] - Mx) * c);
-            sum += m[k] == -INFINITY ? ll[k] : ll[k] * w;  // (a record without weights has m = -inf; its l may be a bad page's NaN)
+            none[k] = m[k] == -INFINITY;
+            const float w = none[k] ? 0.f : __builtin_amdgcn_exp2f((m[k] - Mx) * c);
+            sum += none[k] ? ll[k] : ll[k] * w;  // (a record without weights has m = -inf; its l may be a bad page's NaN)
             m[k] = w;
         }
 #pragma unroll
@@ -860,7 +926,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_flat(const FlatA
             if (e == 0) own[row] = f0 * inv;
 #pragma unroll
             for (int k = 0; k < kMaxParts / 16; ++k)
-                if (e + 16 * k < parts) share[row][e + 16 * k] = m[k] * inv;
+                if (e + 16 * k < parts) share[row][e + 16 * k] = none[k] ? -1.f : m[k] * inv;
         }
         __syncthreads();
     }
@@ -881,8 +947,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_flat(const FlatA
             for (int p = 0; p < parts; ++p) {
                 const float f = share[row][p];
                 const float2 v = *reinterpret_cast<const float2*>(po + p * D);
-                x += f == 0.f ? 0.f : f * v.x;  // (the O of a record without weights is zeros, or of NaN values that have none)
-                y += f == 0.f ? 0.f : f * v.y;
+                x += f < 0.f ? 0.f : f * v.x;  // (the O of a record without weights is zeros, or of NaN values that have none)
+                y += f < 0.f ? 0.f : f * v.y;
             }
             *reinterpret_cast<uint32_t*>(to_out) = pack2<F16>(x, y);
             continue;
