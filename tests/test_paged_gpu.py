@@ -800,3 +800,25 @@ def test_an_infinite_value_of_a_small_weight_gives_an_infinity(dtype, D):
         for x in (a, b, c):
             assert torch.isfinite(x[..., :9].float()).all() and torch.isfinite(x[..., 10:].float()).all()
         assert torch.isfinite(a[:p].float()).all()
+
+
+def test_append_of_more_tokens_than_one_grid_dimension_holds():
+    """2^26 + 5 tokens (four of a workgroup of 256 threads: past 2^32 threads), all but the last five at positions before 0:
+    NaN in their rows; the last five are stored. One row of q, k and v is read for all."""
+    T = (1 << 26) + 5
+    g = _gen(62)
+    x = _rand(g, 1, 1, 64)
+    kc, vc = _cache(g, 1, 1, 16, 64, BF)
+    v0 = vc.clone()
+    cos, sin = _rope(g, 16, 64, BF, False, True)
+    qo = torch.zeros(T, 1, 64, dtype=BF, device=DEV)
+    rows = x.expand(T, 1, 64)
+    kernels.kv_append(rows, rows, rows, cos, sin, _i32([0, T]), _i32([5]), _i32([[0]]), kc, vc, qo=qo)
+    for i in range(0, T - 5, 1 << 23):
+        assert qo[i : min(i + (1 << 23), T - 5)].isnan().all(), i
+    for p in range(5):
+        ref, S = _append_ref(x[0], None, 0.0, cos[p], sin[p], False)
+        _check_append(qo[T - 5 + p], ref, S, BF)
+        _check_append(kc[0, :, p], ref, S, BF)
+        v0[0, :, p] = x[0]
+    assert torch.equal(vc, v0)

@@ -86,7 +86,7 @@ __global__ __launch_bounds__(256) void k_kv_append(const AppendArgs a) {
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int hl = lane & (LPH - 1), hw = lane / LPH, e0 = 8 * hl;
     const int heads = a.hq + 2 * a.hk, groups = (heads + HPW - 1) / HPW;
-    const uint32_t id = blockIdx.x * 4u + wv;
+    const uint32_t id = (blockIdx.y * gridDim.x + blockIdx.x) * 4u + wv;
     const int tok = (int)(id / (uint32_t)a.waves), g0 = (int)(id - (uint32_t)tok * a.waves) * a.per_wave;
     if (tok >= a.T) return;
 
@@ -253,9 +253,9 @@ extern "C" int wisp_kv_append(const void* q, int64_t q_ts, int64_t q_hs, const v
                  (const uint16_t*)q_norm_w, (const uint16_t*)k_norm_w, eps, cos, sin, cs_rows, rot, cu, kv_len, table,
                  width, B, (int)T, hq, hk, per_wave, waves, paged_kv(kc, vc, pages, page, page_stride, head_stride, row_stride),
                  (uint16_t*)qo};
-    const int64_t blocks = (T * waves + 3) / 4;
-    if (blocks > 0x3FFFFFFF) return fail_inval("too many tokens for one call");
-    const dim3 grid((unsigned)blocks);
+    // in two dimensions: one holds fewer than 2^32 threads, 2^24 of these workgroups (what is past them is cut off unseen)
+    const int64_t blocks = (T * waves + 3) / 4, row = 1 << 23;
+    const dim3 grid((unsigned)(blocks < row ? blocks : row), (unsigned)((blocks + row - 1) / row));
     hipStream_t st = (hipStream_t)stream;
     const bool cs32 = cs_dtype == WISP_DT_F32;
     const int in = interleaved ? 2 : rot == d ? 1 : 0;
