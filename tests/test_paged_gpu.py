@@ -822,3 +822,31 @@ def test_append_of_more_tokens_than_one_grid_dimension_holds():
         _check_append(kc[0, :, p], ref, S, BF)
         v0[0, :, p] = x[0]
     assert torch.equal(vc, v0)
+
+
+def test_batch_of_more_rows_than_one_grid_dimension_holds():
+    """2^24 rows (a workgroup of 256 threads each where records are joined: 2^32 threads): sequences without positions among
+    short ones, and a last one long enough to be cut."""
+    B, hq, hk, page, long = 1 << 14, 1024, 64, 2048, 300000
+    g = _gen(63)
+    W = -(-long // page)
+    kc, vc = (_rand(g, 3, hk, page, 64) for _ in range(2))
+    lens = [(7 * i) % 4 for i in range(B - 1)] + [long]
+    table = torch.randint(0, 3, (B, W), generator=g, device=DEV, dtype=torch.int32)
+    q = _rand(g, B, hq, 64)
+    out = torch.full_like(q, 7.0)
+    kernels.attn_batch(q, kc, vc, _i32(lens), table, 0.125, out=out)
+    few = 4000
+    some = kernels.attn_batch(q[:few], kc, vc, _i32(lens[:few]), table[:few].contiguous(), 0.125)
+    assert torch.equal(out[:few], some)
+    some = kernels.attn_batch(q[-few:-1], kc, vc, _i32(lens[-few:-1]), table[-few:-1].contiguous(), 0.125)
+    assert torch.equal(out[-few:-1], some)
+    empty = torch.tensor(lens, device=DEV) == 0
+    assert (out[empty] == 0).all()
+    heads = [0, 5, 63]
+    k, v = (torch.cat([c[table[-1, w].long()][heads] for w in range(W)], 1)[:, :long].double() for c in (kc, vc))
+    rows = torch.cat([q[-1:, 16 * h : 16 * h + 16] for h in heads], 1)
+    p = (torch.matmul(rows.view(3, 16, 64).double(), k.transpose(1, 2).contiguous()) * 0.125).softmax(-1)
+    ref, A = (torch.matmul(p, x).view(1, 48, 64) for x in (v, v.abs()))
+    got = torch.cat([out[-1:, 16 * h : 16 * h + 16] for h in heads], 1)
+    _check(got, ref, A, BF, True)

@@ -995,7 +995,8 @@ __global__ __launch_bounds__(256) void k_attn_join(const JoinArgs a) {
     constexpr int EPL = D / 64;
     __shared__ float rm[4], rl[4], ro[4][D];
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t row = blockIdx.x;
+    const int64_t row = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+    if (row >= (int64_t)a.T * a.hq) return;
     const int tok = (int)(row / a.hq), hd = (int)(row - (int64_t)tok * a.hq);
     int na = 0, nb = 0;
     int64_t a0 = 0;
@@ -1086,10 +1087,13 @@ void launch_flat(const FlatArgs& a, int d, int64_t pieces, hipStream_t st) {
     else hipLaunchKernelGGL((k_attn_flat<F16, 256>), grid, dim3(256), 0, st, a);
 }
 template <bool F16>
-void launch_join(const JoinArgs& a, int d, unsigned grid, hipStream_t st) {
-    if (d == 64) hipLaunchKernelGGL((k_attn_join<F16, 64>), dim3(grid), dim3(256), 0, st, a);
-    else if (d == 128) hipLaunchKernelGGL((k_attn_join<F16, 128>), dim3(grid), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((k_attn_join<F16, 256>), dim3(grid), dim3(256), 0, st, a);
+void launch_join(const JoinArgs& a, int d, hipStream_t st) {
+    // a workgroup per row of out, in two dimensions: one holds fewer than 2^32 threads, 2^24 workgroups
+    const int64_t rows = (int64_t)a.T * a.hq, x = 1 << 23;
+    const dim3 grid((unsigned)(rows < x ? rows : x), (unsigned)((rows + x - 1) / x));
+    if (d == 64) hipLaunchKernelGGL((k_attn_join<F16, 64>), grid, dim3(256), 0, st, a);
+    else if (d == 128) hipLaunchKernelGGL((k_attn_join<F16, 128>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((k_attn_join<F16, 256>), grid, dim3(256), 0, st, a);
 }
 
 // Row tiles that T tokens of B sequences can have: each sequence's last may be partly empty.
@@ -1175,8 +1179,8 @@ extern "C" int wisp_attn_prompt(const void* q, int64_t q_ts, int64_t q_hs, const
     else launch_rows<false>(a, d, bm, (int)slots, st);
     if (parts > 1) {
         JoinArgs j{nullptr, nullptr, nullptr, nullptr, cu, kv_len, ml, po, parts, kPartTiles, bm, B, (int)T, hq, hk, width * page, 0, a.c, (uint16_t*)out};
-        if (dtype == WISP_DT_F16) launch_join<true>(j, d, (unsigned)(T * hq), st);
-        else launch_join<false>(j, d, (unsigned)(T * hq), st);
+        if (dtype == WISP_DT_F16) launch_join<true>(j, d, st);
+        else launch_join<false>(j, d, st);
     }
     return check_launch("k_attn_rows");
 }
@@ -1241,8 +1245,8 @@ extern "C" int wisp_attn_batch(const void* q, int64_t q_ts, int64_t q_hs, const 
     if (f16) launch_flat<true>(f, d, w.pieces, st);
     else launch_flat<false>(f, d, w.pieces, st);
     if (!f.single) {
-        if (f16) launch_join<true>(j, d, (unsigned)(B * hq), st);
-        else launch_join<false>(j, d, (unsigned)(B * hq), st);
+        if (f16) launch_join<true>(j, d, st);
+        else launch_join<false>(j, d, st);
     }
     return check_launch("k_attn_flat");
 }
