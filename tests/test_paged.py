@@ -172,3 +172,19 @@ def test_token_counts_past_any_call_are_refused():
         assert L.wisp_attn_prompt_ws_bytes(T, 1, 32, 4, 128, 64, 256) == -1
         assert _prompt(T=T) == -1
         assert _append(T=T) == -1
+
+
+def test_workspaces_keep_records_aligned():
+    """7 heads and 21 parts (43 tiles of 64 positions): an odd number of records, whose sums begin at a multiple of 16 bytes."""
+    L = _lib.lib()
+    recs = 7 * 21
+    assert L.wisp_attn_prompt_ws_bytes(1, 1, 7, 1, 64, 64, 43) == recs * 8 + 8 + recs * 64 * 4
+    assert L.wisp_attn_batch_ws_bytes(1, 7, 1, 64, 64, 1, 43) == recs * 8 + 8 + recs * 64 * 4
+    assert L.wisp_attn_prompt_ws_bytes(2, 1, 7, 1, 64, 64, 43) == 2 * recs * 8 + 2 * recs * 64 * 4
+
+
+def test_workspace_alignment():
+    for call in (_prompt, _batch):
+        for by in (4, 8):
+            assert call(ws=FAKE + by) == _lib.WISP_EALIGN
+            assert b"ws" in _lib.lib().wisp_last_error()

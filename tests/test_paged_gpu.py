@@ -850,3 +850,16 @@ def test_batch_of_more_rows_than_one_grid_dimension_holds():
     ref, A = (torch.matmul(p, x).view(1, 48, 64) for x in (v, v.abs()))
     got = torch.cat([out[-1:, 16 * h : 16 * h + 16] for h in heads], 1)
     _check(got, ref, A, BF, True)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_an_odd_number_of_records(D):
+    """7 query heads over one, 43 tiles of positions in 21 parts, one row: 147 records."""
+    s = _prompt(64, BF, 7, 1, D, 64, [1], [2700], wider=0)
+    assert s["table"].shape[1] == 43
+    ref, A = _prompt_ref(s, [1], [2700])
+    _check(kernels.attn_prompt(**s), ref, A, BF, False)
+    s = _batch(65, HF, 7, 1, D, 64, [20], prefix=2701)
+    s["prefix_table"] = s["prefix_table"][:43].contiguous()
+    ref, A = _batch_ref(s, [20], 2701)
+    _check(kernels.attn_shared(**s), ref, A, HF, False)

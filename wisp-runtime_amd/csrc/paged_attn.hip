@@ -1115,7 +1115,9 @@ bool takes_whole(int B, int hq, int hk, int64_t positions, bool prefix) {
     return positions <= (groups >= 256 || prefix ? 8 : 4) * kStep;
 }
 
-int64_t rec_bytes(int64_t recs, int d) { return recs * (2 + d) * 4; }
+// Records: m and l of all, then, from a multiple of 16 bytes on (k_attn_rows stores 16 at a time), their O.
+int64_t ml_bytes(int64_t recs) { return (recs * 8 + 15) / 16 * 16; }
+int64_t rec_bytes(int64_t recs, int d) { return ml_bytes(recs) + recs * d * 4; }
 
 struct FlatWs {
     int want;  // pieces that the grain aims at
@@ -1129,7 +1131,7 @@ FlatWs flat_ws(int B, int hq, int hk, int d) {
     w.pieces = w.want + B;
     w.first = 0;
     w.ml = ((int64_t)B * 8 + 15) / 16 * 16;
-    w.po = w.ml + (w.pieces * hq * 8 + 15) / 16 * 16;
+    w.po = w.ml + ml_bytes(w.pieces * hq);
     w.end = w.po + w.pieces * hq * d * 4;
     return w;
 }
@@ -1139,6 +1141,14 @@ bool good_scale(float s) { return s > 0.f && s < INFINITY; }
 int check_q(const void* q, int64_t q_ts, int64_t q_hs, const void* out) {
     if (!aligned(q, 16) || !aligned(out, 16) || q_ts % 8 || q_hs % 8) {
         set_error("q, its strides and out must be 16-byte aligned");
+        return WISP_EALIGN;
+    }
+    return WISP_OK;
+}
+
+int check_ws(const void* ws) {
+    if (!aligned(ws, 16)) {
+        set_error("ws must be 16-byte aligned");
         return WISP_EALIGN;
     }
     return WISP_OK;
@@ -1170,8 +1180,9 @@ extern "C" int wisp_attn_prompt(const void* q, int64_t q_ts, int64_t q_hs, const
     const int64_t slots = row_slots(T, B, hq / hk, bm);
     const int parts = row_parts(slots * hk, (int64_t)page * width);
     if (parts > 1 && !ws) return fail_inval("null workspace");
+    if (int rc = check_ws(ws)) return rc;
     float* ml = (float*)ws;
-    float* po = ml ? ml + 2 * T * hq * parts : nullptr;
+    float* po = ml ? (float*)((uint8_t*)ws + ml_bytes(T * hq * parts)) : nullptr;
     RowsArgs a{(const uint16_t*)q, q_ts, q_hs, paged_kv((void*)kc, (void*)vc, pages, page, page_stride, head_stride, row_stride),
                cu, kv_len, table, width, B, (int)T, hq, hk, hq / hk, 1.f / (float)(hq / hk), scale * 1.44269504088896340736f, parts, kPartTiles, ml, po, (uint16_t*)out};
     hipStream_t st = (hipStream_t)stream;
@@ -1212,10 +1223,7 @@ extern "C" int wisp_attn_batch(const void* q, int64_t q_ts, int64_t q_hs, const 
     const bool whole = takes_whole(B, hq, hk, (int64_t)width * page, prefix_width > 0);
     if (!ws && (!whole || prefix_width)) return fail_inval("null workspace");
     if (int rc = check_q(q, q_ts, q_hs, out)) return rc;
-    if (!aligned(ws, 16)) {
-        set_error("ws must be 16-byte aligned");
-        return WISP_EALIGN;
-    }
+    if (int rc = check_ws(ws)) return rc;
     FlatWs w = flat_ws(B, hq, hk, d);
     if (whole) w.ml = w.po = w.end = 0;  // (no records of its own)
     if ((int64_t)B * hq > (1 << 30) || (int64_t)B * ((int64_t)width * page / kStep + 1) > 0x7FFFFFFF)
@@ -1234,7 +1242,7 @@ extern "C" int wisp_attn_batch(const void* q, int64_t q_ts, int64_t q_hs, const 
         const int parts = prefix_parts(B, hq, hk, d, (int64_t)page * prefix_width);
         float* rml = (float*)(p + w.end);
         RowsArgs a{(const uint16_t*)q, q_ts, q_hs, kv, nullptr, prefix_len, prefix_table, prefix_width, B, B, hq, hk, hq / hk, 1.f / (float)(hq / hk), c, parts, 1,
-                   rml, rml + 2 * (int64_t)B * hq * parts, nullptr};
+                   rml, (float*)((uint8_t*)rml + ml_bytes((int64_t)B * hq * parts)), nullptr};
         if (f16) launch_rows<true>(a, d, bm, slots, st);
         else launch_rows<false>(a, d, bm, slots, st);
         j.rml = f.rml = a.ml;
