@@ -241,7 +241,7 @@ int wisp_kv_append(const void* q, int64_t q_ts, int64_t q_hs, const void* k, int
 
 /* Causal attention of packed tokens over the cache: out[t] [T][hq][d] = softmax(scale q[t] . k[j]) v[j] over the positions
  * j up to t's own; head h reads K/V head h / (hq / hk). A token at a negative position attends nothing and gives zeros.
- * scale positive and finite. ws: wisp_attn_prompt_ws_bytes(T, B, hq, hk, d, page, width) bytes, 16-byte aligned (may be
+ * scale positive, and finite times log2(e). ws: wisp_attn_prompt_ws_bytes(T, B, hq, hk, d, page, width) bytes, 16-byte aligned (may be
  * NULL where that is 0). Where a sequence reads a bad page, rows at and after it are NaN, and rows up to 255 / G tokens
  * before may be. */
 int64_t wisp_attn_prompt_ws_bytes(int64_t T, int B, int hq, int hk, int d, int page, int width);

@@ -188,3 +188,9 @@ def test_workspace_alignment():
         for by in (4, 8):
             assert call(ws=FAKE + by) == _lib.WISP_EALIGN
             assert b"ws" in _lib.lib().wisp_last_error()
+
+
+@pytest.mark.parametrize("call", [_prompt, _batch])
+def test_a_scale_past_the_exponent_is_refused(call):
+    assert call(scale=3e38) == _lib.WISP_EINVAL  # times log2(e): infinite
+    assert b"scale" in _lib.lib().wisp_last_error()

@@ -863,3 +863,16 @@ def test_an_odd_number_of_records(D):
     s["prefix_table"] = s["prefix_table"][:43].contiguous()
     ref, A = _batch_ref(s, [20], 2701)
     _check(kernels.attn_shared(**s), ref, A, HF, False)
+
+
+@pytest.mark.parametrize("scale", [1e-20, 1e-38, 1e-40, 1e-45])
+@pytest.mark.parametrize("dtype,D", [(BF, 64), (HF, 128), (BF, 256)])
+def test_a_scale_next_to_zero_gives_the_mean(scale, dtype, D):
+    lens = [3000, 200, 0]
+    for prefix in (None, 1500):
+        s = dict(_batch(66, dtype, 8, 2, D, 64, lens, prefix=prefix), scale=scale)
+        ref, A = _batch_ref(s, lens, prefix or 0)
+        _check((kernels.attn_shared if prefix else kernels.attn_batch)(**s), ref, A, dtype, not prefix)
+    s = _prompt(67, dtype, 8, 2, D, 64, [5, 70], [3000, 3], scale=scale)
+    ref, A = _prompt_ref(s, [5, 70], [3000, 3])
+    _check(kernels.attn_prompt(**s), ref, A, dtype, False)

@@ -20,6 +20,7 @@
 //               the group), so grouped heads share every K/V tile; all waves walk the same tiles of 64 positions.
 //  k_attn_flat  one query token per sequence: a wave takes the G rows of one K/V head (16 at most), and the four waves
 //               of a workgroup, each with a slot of its own, every fourth 32 positions. HBM-bound.
+#include <float.h>
 #include <math.h>
 
 #include "paged.hpp"
@@ -44,6 +45,9 @@ constexpr int kStep = 4 * kSub;    // positions of a workgroup's four slots: the
 constexpr float kLazy = 6.f;       // m follows the maximum past 2^kLazy
 constexpr int kSlotsY = 32768;     // grid.y of k_attn_rows
 constexpr int kMaxParts = 64;       // parts of a shared prefix
+
+// The step of the maximum past m, in scores, that m follows. (Finite: -inf, where m begins, plus an infinite step is NaN.)
+__device__ __forceinline__ float follow(float c) { return fminf(kLazy / c, FLT_MAX); }
 
 // float16 weights p: times 2^8, so that small ones keep their bits (the grain 2^-24 is then 2^-32 of the largest) and
 // 2^(8 + kLazy) stays below the type's 65,504. bfloat16 has binary32's range.
@@ -385,7 +389,7 @@ __global__ __launch_bounds__(64 * NW, D == 64 && NW == 4 ? 3 : 1) void k_attn_ro
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
     float m = -INFINITY, mb = 0.f, l = 0.f;  // reference, c * m - bias (0 while m is -inf), this lane's share of the sum
-    const float c = a.c, th = kLazy / a.c;
+    const float c = a.c, th = follow(a.c);
     uint4 pb[4];  // B operand of positions 16 ks ..: slot 8 hf + e is position 16 ks + 8 (e/4) + 4 hf + e%4
 
     auto scores = [&](int j) {  // S(j)
@@ -778,7 +782,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_flat(const FlatA
 #pragma unroll
     for (int d = 0; d < ND; ++d) o[d] = f4_t{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, mb = 0.f, l = 0.f;
-    const float c = a.c, th = kLazy / a.c;
+    const float c = a.c, th = follow(a.c);
     for (int p = p_first; p < to; p += kStep) {
         const bool more = p + kStep < to;
         wait_vm<LI>();  // K is there, V may be in flight
@@ -1136,7 +1140,8 @@ FlatWs flat_ws(int B, int hq, int hk, int d) {
     return w;
 }
 
-bool good_scale(float s) { return s > 0.f && s < INFINITY; }
+constexpr float kLog2E = 1.44269504088896340736f;
+bool good_scale(float s) { return s > 0.f && s * kLog2E < INFINITY; }
 
 int check_q(const void* q, int64_t q_ts, int64_t q_hs, const void* out) {
     if (!aligned(q, 16) || !aligned(out, 16) || q_ts % 8 || q_hs % 8) {
@@ -1172,7 +1177,7 @@ extern "C" int wisp_attn_prompt(const void* q, int64_t q_ts, int64_t q_hs, const
     clear_error();
     if (int rc = check_paged(kc, vc, pages, page, page_stride, head_stride, row_stride, width, B, hq, hk, d, dtype)) return rc;
     if (T < 0 || T > (1 << 30) || T * hq > (1 << 30)) return fail_inval("T * hq must be in [0, 2^30]");
-    if (!good_scale(scale)) return fail_inval("scale must be positive and finite");
+    if (!good_scale(scale)) return fail_inval("scale must be positive, and finite times log2(e)");
     if (T == 0) return WISP_OK;
     if (!q || !cu || !kv_len || !table || !out) return fail_inval("null pointer");
     if (int rc = check_q(q, q_ts, q_hs, out)) return rc;
@@ -1184,7 +1189,7 @@ extern "C" int wisp_attn_prompt(const void* q, int64_t q_ts, int64_t q_hs, const
     float* ml = (float*)ws;
     float* po = ml ? (float*)((uint8_t*)ws + ml_bytes(T * hq * parts)) : nullptr;
     RowsArgs a{(const uint16_t*)q, q_ts, q_hs, paged_kv((void*)kc, (void*)vc, pages, page, page_stride, head_stride, row_stride),
-               cu, kv_len, table, width, B, (int)T, hq, hk, hq / hk, 1.f / (float)(hq / hk), scale * 1.44269504088896340736f, parts, kPartTiles, ml, po, (uint16_t*)out};
+               cu, kv_len, table, width, B, (int)T, hq, hk, hq / hk, 1.f / (float)(hq / hk), scale * kLog2E, parts, kPartTiles, ml, po, (uint16_t*)out};
     hipStream_t st = (hipStream_t)stream;
     if (dtype == WISP_DT_F16) launch_rows<true>(a, d, bm, (int)slots, st);
     else launch_rows<false>(a, d, bm, (int)slots, st);
@@ -1217,7 +1222,7 @@ extern "C" int wisp_attn_batch(const void* q, int64_t q_ts, int64_t q_hs, const 
                                float scale, void* ws, void* out, void* stream) {
     clear_error();
     if (int rc = check_paged(kc, vc, pages, page, page_stride, head_stride, row_stride, width, B, hq, hk, d, dtype)) return rc;
-    if (!good_scale(scale)) return fail_inval("scale must be positive and finite");
+    if (!good_scale(scale)) return fail_inval("scale must be positive, and finite times log2(e)");
     if (prefix_width < 0 || (int64_t)prefix_width * page > (1 << 30)) return fail_inval("the prefix's positions must be in [0, 2^30]");
     if (!q || !kv_len || !table || !out || (prefix_width && (!prefix_len || !prefix_table))) return fail_inval("null pointer");
     const bool whole = takes_whole(B, hq, hk, (int64_t)width * page, prefix_width > 0);
@@ -1229,7 +1234,7 @@ extern "C" int wisp_attn_batch(const void* q, int64_t q_ts, int64_t q_hs, const 
     if ((int64_t)B * hq > (1 << 30) || (int64_t)B * ((int64_t)width * page / kStep + 1) > 0x7FFFFFFF)
         return fail_inval("too many sequences, or positions in their tables, for one call");
     const PagedKV kv = paged_kv((void*)kc, (void*)vc, pages, page, page_stride, head_stride, row_stride);
-    const float c = scale * 1.44269504088896340736f;
+    const float c = scale * kLog2E;
     uint8_t* p = (uint8_t*)ws;
     hipStream_t st = (hipStream_t)stream;
     const bool f16 = dtype == WISP_DT_F16;
