@@ -194,3 +194,24 @@ def test_workspace_alignment():
 def test_a_scale_past_the_exponent_is_refused(call):
     assert call(scale=3e38) == _lib.WISP_EINVAL  # times log2(e): infinite
     assert b"scale" in _lib.lib().wisp_last_error()
+
+
+def test_strides_of_dimensions_of_size_one_say_nothing():
+    bf = torch.bfloat16
+    x = torch.zeros(40000, dtype=bf)
+    for t, want in ((x.as_strided((1, 8, 128), (4097, 128, 1)), 128), (x.as_strided((1, 8, 128), (4097, 136, 1)), 136)):
+        y, at, ts, hs = kernels._rows(t, "q")
+        assert at == t.data_ptr() and ts % 8 == 0 and hs == want  # as it is
+    y, at, ts, hs = kernels._rows(x.as_strided((5, 1, 128), (136, 3, 1)), "q")
+    assert at == x.data_ptr() and ts == 136 and hs % 8 == 0
+    y, at, ts, hs = kernels._rows(x.as_strided((1, 8, 128), (4097, 132, 1)), "q")
+    assert at != x.data_ptr() and (ts, hs) == (1024, 128)  # a copy
+    y, at, ts, hs = kernels._rows(x[4:].as_strided((1, 8, 128), (4097, 128, 1), 4), "q")
+    assert at % 16 == 0 and at != x.data_ptr() + 8 and (ts, hs) == (1024, 128)
+    q, table = torch.zeros(1, 8, 128, dtype=bf), torch.zeros(1, 1, dtype=torch.int32)
+    one_page = x.as_strided((1, 2, 64, 128), (16385, 8192, 128, 1)), x.as_strided((1, 2, 64, 128), (7, 8192, 128, 1))
+    assert kernels._paged_cache(q, *one_page, table, "t")[4][4:] == (0, 8192, 128)
+    one_head = x.as_strided((3, 1, 64, 128), (8192, 3, 128, 1)), x.as_strided((3, 1, 64, 128), (8192, 8192, 128, 1))
+    assert kernels._paged_cache(q, *one_head, table, "t")[4][4:] == (8192, 0, 128)
+    with pytest.raises(AssertionError):
+        kernels._paged_cache(q, one_head[0], x.as_strided((3, 1, 64, 128), (8704, 8192, 136, 1)), table, "t")

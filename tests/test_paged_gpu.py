@@ -876,3 +876,27 @@ def test_a_scale_next_to_zero_gives_the_mean(scale, dtype, D):
     s = _prompt(67, dtype, 8, 2, D, 64, [5, 70], [3000, 3], scale=scale)
     ref, A = _prompt_ref(s, [5, 70], [3000, 3])
     _check(kernels.attn_prompt(**s), ref, A, dtype, False)
+
+
+def _odd_ones(x, pitch=4097):
+    """x with the strides of its dimensions of size 1 replaced by an odd number."""
+    return x.as_strided(x.shape, [pitch if n == 1 else s for n, s in zip(x.shape, x.stride())])
+
+
+@pytest.mark.parametrize("hq,hk", [(8, 1), (1, 1), (8, 2)])
+def test_odd_strides_of_dimensions_of_size_one(hq, hk):
+    """One token, one head, one page: strides that no address is formed with, as torch leaves them after a cut."""
+    g = _gen(68)
+    kc, vc = _cache(g, 1, hk, 64, 128, BF)
+    q, k, v = _rand(g, 1, hq, 128), _rand(g, 1, hk, 128), _rand(g, 1, hk, 128)
+    cos, sin = _rope(g, 64, 128, BF, False, False)
+    one, zero = _i32([30]), _i32([[0]])
+    caches = [[c.clone() for c in (kc, vc)] for _ in range(2)]
+    res = []
+    for odd, (a, b) in zip((lambda x: x, _odd_ones), caches):
+        q1 = kernels.kv_append(odd(q), odd(k), odd(v), cos, sin, _i32([0, 1]), one, zero, odd(a), b)
+        res.append([q1, kernels.attn_prompt(odd(q), a, odd(b), _i32([0, 1]), one, zero, 0.1),
+                    kernels.attn_batch(odd(q1), odd(a), b, one, zero, 0.1),
+                    kernels.attn_shared(odd(q1), odd(a), odd(b), one, zero, one, zero[0], 0.1), a, b])
+    for x, y in zip(*res):
+        assert torch.equal(x, y)

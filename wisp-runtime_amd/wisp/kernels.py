@@ -558,10 +558,12 @@ def _paged_cache(q, kc, vc, table, what):
     dt = _CACHE_DTYPES.get(dtype)
     if dt is None or kc.dtype != dtype or vc.dtype != dtype:
         raise TypeError(f"{what} takes bfloat16 or float16 of one dtype (got {dtype}, {kc.dtype}, {vc.dtype})")
-    shape, st = kc.shape, kc.stride()
+    shape, st, sv = kc.shape, kc.stride(), vc.stride()
     assert len(shape) == 4 and shape == vc.shape and shape[3] == D, "caches must be [pages, Hk, page, D]"
-    assert st[3] == 1 and st == vc.stride(), "caches need contiguous rows and equal strides"
     P, hk, page, _ = shape
+    if P == 1 or hk == 1:  # the stride of a dimension of size 1 says nothing
+        st, sv = (tuple(0 if n == 1 else x for n, x in zip(shape, s)) for s in (st, sv))
+    assert st[3] == 1 and st == sv, "caches need contiguous rows and equal strides"
     assert hq % hk == 0, f"{hq} query heads over {hk} K/V heads"
     if table.dtype != torch.int32 or table.dim() != 2 or not table.is_contiguous():
         raise TypeError("table must be a contiguous int32 [B, pages of a sequence] tensor")
@@ -574,12 +576,14 @@ def _rows(x, what):
     that the kernels read."""
     st = x.stride()
     assert len(st) == 3, f"{what} must be [tokens, heads, D]"
-    if st[2] != 1 or st[0] % 8 or st[1] % 8 or x.data_ptr() % 16:
+    T, h, D = x.shape
+    ts, hs = 0 if T == 1 else st[0], 0 if h == 1 else st[1]  # (the stride of a dimension of size 1 says nothing)
+    if st[2] != 1 or ts % 8 or hs % 8 or x.data_ptr() % 16:
         x = x.contiguous()
         if x.data_ptr() % 16:
             x = x.clone()
-        st = x.stride()
-    return x, x.data_ptr(), st[0], st[1]
+        ts, hs = h * D, D
+    return x, x.data_ptr(), ts, hs
 
 
 def _out(out, shape, like):
