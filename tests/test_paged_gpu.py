@@ -900,3 +900,46 @@ def test_odd_strides_of_dimensions_of_size_one(hq, hk):
                     kernels.attn_shared(odd(q1), odd(a), odd(b), one, zero, one, zero[0], 0.1), a, b])
     for x, y in zip(*res):
         assert torch.equal(x, y)
+
+
+def test_no_sequences():
+    g = _gen(69)
+    kc, vc = _cache(g, 4, 2, 16, 128, BF)
+    k0, v0 = kc.clone(), vc.clone()
+    cos, sin = _rope(g, 8, 128, BF, False, False)
+    none = torch.empty(0, dtype=torch.int32, device=DEV)
+    for W in (0, 3):
+        table = torch.zeros(0, W, dtype=torch.int32, device=DEV)
+        q = _rand(g, 0, 8, 128)
+        assert kernels.attn_batch(q, kc, vc, none, table, 0.1).shape == (0, 8, 128)
+        for pre in (none, _i32([1])):
+            assert kernels.attn_shared(q, kc, vc, none, table, _i32([3]), pre, 0.1).shape == (0, 8, 128)
+        for T in (0, 5):  # five rows that belong to no sequence
+            q, k, out = _rand(g, T, 8, 128), _rand(g, T, 2, 128), torch.full((T, 8, 128), 2.0, dtype=BF, device=DEV)
+            assert kernels.kv_append(q, k, k, cos, sin, _i32([0]), none, table, kc, vc, qo=out) is out and (out == 2.0).all()
+            assert kernels.attn_prompt(q, kc, vc, _i32([0]), none, table, 0.1, out=out) is out and (out == 2.0).all()
+    assert torch.equal(kc, k0) and torch.equal(vc, v0)
+
+
+def test_tables_without_pages():
+    """Sequences of length 0 read nothing; a length past such a table is NaN, as past any."""
+    s = _batch(70, BF, 8, 2, 128, 16, [0, 0, 40], prefix=70)
+    table = torch.empty(3, 0, dtype=torch.int32, device=DEV)
+    none = dict(s, table=table, kv_len=_i32([0, 0, 1]))
+    got = kernels.attn_shared(**none)
+    want = kernels.attn_shared(**dict(s, kv_len=_i32([0, 0, 0])))
+    assert torch.equal(got[:2], want[:2]) and got[2].isnan().all()
+    got = kernels.attn_shared(**dict(s, prefix_table=table[0], prefix_len=_i32([0])))
+    own = {k: v for k, v in s.items() if not k.startswith("prefix")}
+    ref, A = _batch_ref(own, [0, 0, 40])
+    _check(got, ref, A, BF, False)
+    assert kernels.attn_shared(**dict(s, prefix_table=table[0])).isnan().all()
+    got = kernels.attn_batch(**dict(own, table=table, kv_len=_i32([0, 5, -1])))
+    assert (got[0] == 0).all() and got[1].isnan().all() and (got[2] == 0).all()
+    q, k = _rand(_gen(71), 2, 8, 128), _rand(_gen(72), 2, 2, 128)
+    cos, sin = _rope(None, 8, 128, BF, False, False)
+    k0 = s["kc"].clone()
+    assert kernels.kv_append(q, k, k, cos, sin, _i32([0, 2, 2, 2]), _i32([2, 0, 0]), table, s["kc"], s["vc"]).isnan().all()
+    assert torch.equal(s["kc"], k0)
+    got = kernels.attn_prompt(q, s["kc"], s["vc"], _i32([0, 2, 2, 2]), _i32([0, 0, 0]), table, 0.1)  # positions -2 and -1
+    assert (got == 0).all()

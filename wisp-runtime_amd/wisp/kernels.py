@@ -552,7 +552,7 @@ def _int32(t, n, what):
 
 def _paged_cache(q, kc, vc, table, what):
     """Checks of a paged cache and its tables against q [.., hq, D]: (WISP_DT_* code, B, table width, K/V heads, the C entry
-    points' cache arguments)."""
+    points' cache arguments, the table: where it holds no pages, one of a page that does not exist)."""
     _, hq, D = q.shape
     dtype = q.dtype
     dt = _CACHE_DTYPES.get(dtype)
@@ -568,7 +568,14 @@ def _paged_cache(q, kc, vc, table, what):
     if table.dtype != torch.int32 or table.dim() != 2 or not table.is_contiguous():
         raise TypeError("table must be a contiguous int32 [B, pages of a sequence] tensor")
     B, width = table.shape
-    return dt, B, width, hk, (kc.data_ptr(), vc.data_ptr(), P, page, st[0], st[1], st[2])
+    if width == 0:
+        table, width = _no_pages(table, (B, 1)), 1
+    return dt, B, width, hk, (kc.data_ptr(), vc.data_ptr(), P, page, st[0], st[1], st[2]), table
+
+
+def _no_pages(table, shape):
+    """What a table without pages means to the kernels: lengths of 0 read nothing, others are past it (NaN)."""
+    return torch.full(shape, -1, dtype=torch.int32, device=table.device)
 
 
 def _rows(x, what):
@@ -618,7 +625,7 @@ def kv_append(q, k, v, cos, sin, cu, kv_len, table, kc, vc, q_norm_w=None, k_nor
     pairs (i, i + R/2), or (2i, 2i + 1) where interleaved. float32 throughout, rounded once.
     Returns the rotated q [T, Hq, D]; its rows from cu[B] on are left as they were (qo) or undefined."""
     T, hq, D = q.shape
-    dt, B, width, hk, cache = _paged_cache(q, kc, vc, table, "kv_append")
+    dt, B, width, hk, cache, table = _paged_cache(q, kc, vc, table, "kv_append")
     dtype = q.dtype
     assert (q_norm_w is None) == (k_norm_w is None), "q_norm_w and k_norm_w: both or neither"
     norms = () if q_norm_w is None else (q_norm_w, k_norm_w)
@@ -636,6 +643,8 @@ def kv_append(q, k, v, cos, sin, cu, kv_len, table, kc, vc, q_norm_w=None, k_nor
     v, vp, v_ts, v_hs = _rows(v, "v")
     cos, sin = cos.contiguous(), sin.contiguous()
     qo = _out(qo, (T, hq, D), q)
+    if B == 0:
+        return qo
     qw, kw = (w.data_ptr() for w in norms) if norms else (None, None)
     rows, rot = cos.shape
     _call(dev, _lib.lib().wisp_kv_append,
@@ -652,12 +661,14 @@ def attn_prompt(q, kc, vc, cu, kv_len, table, scale, out=None):
     were (out) or undefined. Nothing is read back to the host, so the call can be captured and the lengths changed between
     replays."""
     T, hq, D = q.shape
-    dt, B, width, hk, cache = _paged_cache(q, kc, vc, table, "attn_prompt")
+    dt, B, width, hk, cache, table = _paged_cache(q, kc, vc, table, "attn_prompt")
     dev = _lib.require_gpu(q, kc, vc, cu, kv_len, table, what="attn_prompt")
     _int32(cu, B + 1, "cu")
     _int32(kv_len, B, "kv_len")
     q, qp, q_ts, q_hs = _rows(q, "q")
     out = _out(out, (T, hq, D), q)
+    if B == 0:
+        return out
     L = _lib.lib()
     nb = L.wisp_attn_prompt_ws_bytes(T, B, hq, hk, D, cache[3], width)
     ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb > 0 else None
@@ -669,7 +680,7 @@ def attn_prompt(q, kc, vc, cu, kv_len, table, scale, out=None):
 
 def _attn_batch(q, kc, vc, kv_len, table, prefix, scale, out, what):
     n, hq, D = q.shape
-    dt, B, width, hk, cache = _paged_cache(q, kc, vc, table, what)
+    dt, B, width, hk, cache, table = _paged_cache(q, kc, vc, table, what)
     assert B == n, f"{n} rows of q, {B} of table"
     dev = _lib.require_gpu(q, kc, vc, kv_len, table, *prefix, what=what)
     _int32(kv_len, B, "kv_len")
@@ -679,10 +690,14 @@ def _attn_batch(q, kc, vc, kv_len, table, prefix, scale, out, what):
         pw = ptable.numel()
         _int32(plen, 1, "prefix_len")
         _int32(ptable, pw, "prefix_table")
-        assert ptable.dim() == 1 and pw >= 1, "prefix_table must be [pages of the prefix]"
+        assert ptable.dim() == 1, "prefix_table must be [pages of the prefix]"
+        if pw == 0:
+            ptable, pw = _no_pages(ptable, (1,)), 1
         pre = (plen.data_ptr(), ptable.data_ptr(), pw)
     q, qp, q_ts, q_hs = _rows(q, "q")
     out = _out(out, (B, hq, D), q)
+    if B == 0:
+        return out
     L = _lib.lib()
     nb = L.wisp_attn_batch_ws_bytes(B, hq, hk, D, cache[3], width, pre[2])
     ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb > 0 else None
