@@ -413,3 +413,40 @@ def test_prefill_of_two_gib_of_tokens(bits, H, I):
         a = (torch.nn.functional.silu(xs @ g.t()) * (xs @ u.t())).to(torch.bfloat16).float()
         ref += (sel[some] == e) * rw[some] * (a @ d.t())
     assert ((got[some].float() - ref).norm() / ref.norm()).item() <= 2.0**-7
+
+
+@pytest.mark.parametrize("Hq,Hk,D", [(32, 4, 128), (4, 4, 64), (16, 2, 256), (32, 2, 128), (8, 4, 256)])
+def test_attn_decode_of_an_infinite_value_is_infinite(Hq, Hk, D):
+    """An infinity in V that the token attends (its own position's among them, which the last rows of a chunk repeat): the
+    infinity in its dim, every other dim as without it, bit for bit; NaN for both signs or a NaN; nothing where it lies past
+    the position. dl_qk_rope_attn the same."""
+    T, pos = 512, 300
+    g = torch.Generator(device=DEV).manual_seed(Hq + D)
+    rand = lambda *shape: torch.randn(shape, generator=g, device=DEV).to(torch.bfloat16)
+    q, k, v, p = rand(Hq, D), rand(1, Hk, T, D), rand(1, Hk, T, D), torch.tensor([pos], device=DEV)
+    qkv, w = rand((Hq + 2 * Hk) * D), rand(D)
+    ang = torch.rand(T, D, generator=g, device=DEV)
+    cos, sin = ang.cos().to(torch.bfloat16), ang.sin().to(torch.bfloat16)
+
+    def both(v, own=None):
+        x = qkv.clone()
+        if own is not None:
+            x.view(-1, D)[Hq + Hk :, 7] = own
+        a = kernels.attn_decode(q, k, v, p, D**-0.5).view(Hq, D)
+        return a, kernels.dl_qk_rope_attn(x, w, w, 1e-6, cos, sin, p, Hq, Hk, D, k.clone(), v.clone(), D**-0.5).view(Hq, D)
+
+    want = both(v)
+    rest = [d for d in range(D) if d != 7]
+    for at in (0, 17, 63, 64, 255, pos):
+        for value in (float("inf"), -float("inf"), float("nan")):
+            x = v.clone()
+            x[0, :, at, 7] = value
+            for got, ref in zip(both(x, value if at == pos else None), want):
+                hit = got[:, 7]
+                assert (hit.isnan() if value != value else hit == value).all(), (at, value)
+                assert torch.equal(got[:, rest], ref[:, rest])
+    x = v.clone()
+    x[0, :, 20, 7], x[0, :, 25, 7] = float("inf"), -float("inf")
+    x[0, :, pos + 1 :, 9] = float("inf")
+    for got, ref in zip(both(x), want):
+        assert got[:, 7].isnan().all() and torch.equal(got[:, rest], ref[:, rest])
