@@ -1,6 +1,8 @@
 """GraphDecoder.prefill(fused=True): the decoder's prompts through kv_append and attn_prompt, on the small Qwen3-MoE of
 test_graphdec_gpu.py, with that file's bar against transformers in float32 (the bf16 roundings of three layers)."""
 
+from types import SimpleNamespace
+
 import pytest
 import torch
 
@@ -66,3 +68,44 @@ def test_turns_of_fused_and_plain_prefill_share_the_cache():
         err, ok = _close(dec.prefill(ids[0, 12:].cuda(), 12, chunk=3, fused=True), want, 2e-2)
     assert ok, err
     rt.cache.free()
+
+
+@pytest.mark.parametrize("turns", [[1500], [700, 1, 640]])
+def test_fused_attention_at_length(turns):
+    """Layer 0's attention over the static cache, 32 query and 4 K/V heads of 128, in one piece and in turns: against 64 bits
+    over the keys and values that it stored, with the bound of test_paged_gpu.py."""
+    from test_paged_gpu import _attend, _check, _i32
+
+    from wisp import kernels
+
+    Hq, Hk, D, hid, T = 32, 4, 128, 256, sum(turns)
+    g = torch.Generator(device="cuda").manual_seed(7)
+    rand = lambda *s: (torch.randn(s, generator=g, device="cuda") * hid**-0.5).to(torch.bfloat16)
+    lin = [torch.nn.Linear(hid, h * D, bias=False, device="cuda", dtype=torch.bfloat16) for h in (Hq, Hk, Hk)]
+    with torch.no_grad():
+        for m in lin:
+            m.weight.copy_(rand(*m.weight.shape))
+    at = SimpleNamespace(q_proj=lin[0], k_proj=lin[1], v_proj=lin[2])
+    w = dict(qn=rand(D) + 1, kn=rand(D) + 1, epsq=1e-6, scale=D**-0.5)
+    cap = -(-T // 64) * 64 + 64
+    ang = torch.rand(cap, D // 2, generator=g, device="cuda").repeat(1, 2)
+    dec = SimpleNamespace(shape=SimpleNamespace(per_layer=[w]), D=D, Hq=Hq, Hk=Hk, cos=ang.cos().to(torch.bfloat16),
+                          sin=ang.sin().to(torch.bfloat16), kv=torch.zeros(1, 2, Hk, cap, D, dtype=torch.bfloat16, device="cuda"))
+    x = rand(1, T, hid) * hid**0.5
+    table, done, got, qs = torch.arange(cap // 64, dtype=torch.int32, device="cuda")[None], 0, [], []
+    with torch.no_grad():
+        for n in turns:
+            xn, cu, kv_len = x[:, done : done + n], _i32([0, n]), _i32([done + n])
+            got.append(GraphDecoder._attend_fused(dec, 0, at, xn, cu, kv_len, table).view(n, Hq, D))
+            q, k, v = (m(xn).view(n, -1, D) for m in lin)
+            other = [torch.zeros(cap // 64, Hk, 64, D, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+            qs.append(kernels.kv_append(q, k, v, dec.cos, dec.sin, cu, kv_len, table, *other, w["qn"], w["kn"], 1e-6))
+            stored = [c.transpose(0, 1).reshape(Hk, cap, D)[:, done : done + n] for c in other]
+            for j in range(2):
+                assert torch.equal(dec.kv[0, j, :, done : done + n], stored[j])
+            done += n
+    assert (dec.kv[0, :, :, T:] == 0).all()
+    rows = sorted({0, 1, 63, 64, 255, 256, 699, 700, 701, T // 2, T - 2, T - 1})
+    kk, vv = dec.kv[0, 0, :, :T].double(), dec.kv[0, 1, :, :T].double()
+    ref, A = _attend(torch.cat(qs)[rows], kk, vv, w["scale"], rows)
+    _check(torch.cat(got)[rows], ref, A, torch.bfloat16, False)
