@@ -220,9 +220,10 @@ int wisp_moe_prefill_routed(const uint8_t* pool, int64_t slot_bytes, int64_t nsl
  * page a power of two >= 16; d 64, 128 or 256. Position p of sequence b is row p % page of page
  * table[b * width + p / page] (int32). kv_len[b]: the positions that b has, its new tokens' included. Packed tokens:
  * those of sequence b are rows [cu[b], cu[b + 1]) of q, k, v and the output (cu int32 [B + 1], ascending from 0); the
- * j-th of n is at position kv_len[b] - n + j; rows from cu[B] on are neither read nor written. cu, kv_len and table are
- * device memory, read when the kernels run. A page id outside [0, pages), or a position past the table, is not
- * dereferenced: what depends on it is NaN. No reference counterpart (the reference decodes one sequence).
+ * j-th of n is at position kv_len[b] - n + j; rows from cu[B] on are not written, and belong to no sequence (q, k and v
+ * have all T rows: wisp_kv_append may read them). B and width are 1 at least. cu, kv_len and table are device memory, read
+ * when the kernels run. A page id outside [0, pages), or a position past the table, is not dereferenced: what depends on it
+ * is NaN. No reference counterpart (the reference decodes one sequence).
  *
  * wisp_kv_append: RMSNorm of every q and k head (q_norm_w, k_norm_w [d], or both NULL: none), rotation of the first rot
  * elements of each (rot a multiple of 16, at most d; pairs (i, i + rot/2), or (2i, 2i + 1) with interleaved) with row p of
@@ -241,8 +242,10 @@ int wisp_kv_append(const void* q, int64_t q_ts, int64_t q_hs, const void* k, int
 
 /* Causal attention of packed tokens over the cache: out[t] [T][hq][d] = softmax(scale q[t] . k[j]) v[j] over the positions
  * j up to t's own; head h reads K/V head h / (hq / hk). A token at a negative position attends nothing and gives zeros.
- * scale positive, and finite times log2(e). ws: wisp_attn_prompt_ws_bytes(T, B, hq, hk, d, page, width) bytes, 16-byte aligned (may be
- * NULL where that is 0). Where a sequence reads a bad page, rows at and after it are NaN, and rows up to 255 / G tokens
+ * scale positive, and finite times log2(e). Sums in binary32; the softmax weights that multiply v are rounded to dtype (those
+ * of wisp_attn_batch's own positions to two terms of it), the result once. An infinite value that is attended gives that
+ * infinity. ws: wisp_attn_prompt_ws_bytes(T, B, hq, hk, d, page, width) bytes, 16-byte aligned (may be NULL where that is
+ * 0). Where a sequence reads a bad page, rows at and after it are NaN, and rows up to 255 / G tokens
  * before may be. */
 int64_t wisp_attn_prompt_ws_bytes(int64_t T, int B, int hq, int hk, int d, int page, int width);
 int wisp_attn_prompt(const void* q, int64_t q_ts, int64_t q_hs, const void* kc, const void* vc, int64_t pages, int page,

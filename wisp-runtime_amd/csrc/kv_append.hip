@@ -97,7 +97,7 @@ __global__ __launch_bounds__(256) void k_kv_append(const AppendArgs a) {
                                               : a.v + tok * a.v_ts + (h - a.hq - a.hk) * a.v_hs;
         return *reinterpret_cast<const uint4*>(x + e0);
     };
-    uint4 next = load(g0);
+    uint4 next = load(g0);  // (before it is known whether the row belongs to a sequence: the rows of q, k and v are all there)
 
     // the token's sequence: the one whose range ends past it first; 64 ends are looked at together
     int b = 0, t1 = 0, len = 0;
@@ -243,8 +243,10 @@ extern "C" int wisp_kv_append(const void* q, int64_t q_ts, int64_t q_hs, const v
     const int hpw = 512 / d, groups = (hq + 2 * hk + hpw - 1) / hpw;
     // Few tokens: a wave per head group, so that the call has as many requests in flight as it can. Enough for a wave each
     // to fill most of the 8,192 that the card holds: a wave walks all its token's groups and finds cos, sin and the page
-    // once (6,976 tokens of 40 heads: 34.6 -> 31.3 us). Between them, two to three times the card's waves (4,153 tokens of
-    // 20 heads of 256: 23.1 us; 24.3 with one wave a token, 25.4 with two, just past a full round).
+    // once. Between them, two to three times the card's waves. Groups a wave 1, 2, 4 and all, inputs not in the cache: 10 groups
+    // a token (40 heads of 128, 80 of 64 or 20 of 256 alike) 500 tokens 5.7, 6.0, 7.3, 10.9 us, 1,500 12.7, 11.5, 12.4, 17.9,
+    // 4,500 29.6, 25.0, 26.2, 26.1, 6,143 38.3, 32.1, 34.0, 31.7, 20,000 116, 91, 91, 92; 3 groups (12 heads of 128) 4,500 12.1,
+    // 12.1, -, 11.1, 8,000 17.7, 17.1, -, 16.0; 20 groups (80 heads of 128) 8,000 92, 74, 73, 80: so wide, four would be better.
     int per_wave = 1;
     if (T >= 6144) per_wave = groups;
     while (per_wave < groups && T * ((groups + 2 * per_wave - 1) / (2 * per_wave)) >= 16384) per_wave *= 2;

@@ -4,6 +4,13 @@
 //     o_i = sum_{j <= lim_i} softmax_j(scale q_i . k_j) v_j
 //
 // with G = Hq/Hk query heads per K/V head, q . k and all sums in binary32 from the stored 16-bit values, o rounded once.
+// The weights are rounded, too, as the matrix cores take 16-bit operands: k_attn_rows gives each as one value of the type,
+// which moves o by half a step of it times sum |p v| / l at most; k_attn_flat, bound by HBM, as two, whose sum is the weight
+// to 2^-17 (bfloat16). Against 64 bits (relative, of all outputs): prompts in bfloat16 0.0020, where the rounding of o alone
+// gives 0.0016, and 0.0023 to 0.0017 behind a shared prefix (float16 0.00029 to 0.00021); two terms there would give the
+// smaller figures, for 2,519 us instead of 1,839 at 16,384 tokens, 316 to 241 in a pack of seven prompts and 48.8 to 43.2 for
+// 64 sequences behind 16,000 positions. l is the sum of the unrounded weights: that of the rounded ones changes those errors
+// by 1 % and, at heads of 64, costs 4 % of the time.
 // A row that may attend nothing (lim_i < 0) gives zeros. One pass over the positions with a running reference m: with
 // p_j = 2^(c (s_j - m)), c = scale log2(e), the sums l = sum p_j and O = sum p_j v_j are kept, and multiplied by
 // 2^(c (m_old - m_new)) when m moves. m need not be the maximum, only near it: it follows when the maximum has passed it
@@ -281,9 +288,11 @@ __device__ __forceinline__ bool find_tile(const RowsArgs& a, int s, int lane, Ro
 // two halves of the workgroup take turns: while waves 0-3 run a tile's matrix products, waves 4-7 weigh their tile, and
 // a barrier swaps the parts. A turn M(j) is O += V(j) P(j), then S(j + 1) = K(j + 1) Q^T; a turn W(j) turns S(j) into
 // P(j). K and V of four tiles are in LDS or on their way.
-// Measured (32 query, 4 K/V heads of 128, bfloat16): 16,384 tokens 1,870 us, 1.17 PFLOP/s with the matrix cores 66 % busy at
-// the clock that the power limit leaves; one tile at a time without turns 2,305. 64 query, 8 K/V heads of 64, 1,018 tokens
-// behind 24,000: 400 us, bound by the exponentials. 16 query, 8 K/V heads of 256, 16,000 tokens: 2,230 us, 0.94 PFLOP/s.
+// Measured (32 query, 4 K/V heads of 128, bfloat16): 16,384 tokens 1,840 us, 1.20 PFLOP/s with the matrix cores 67 % and the
+// VALU 58 % busy at the clock that the power limit leaves; one tile at a time without turns 2,305. 64 query, 8 K/V heads of
+// 64, 1,018 tokens behind 24,000: 407 us, matrix cores 41 %, VALU 62 %, 28 % of the waves' time in waits: neither is full, the
+// halves wait for each other. 16 query, 8 K/V heads of 256, 16,000 tokens: 2,230 us, 0.94 PFLOP/s, matrix cores 40 % (one wave
+// a SIMD: weights and products by turns).
 template <bool F16, int D, int NW>
 __global__ __launch_bounds__(64 * NW, D == 64 && NW == 4 ? 3 : 1) void k_attn_rows(const RowsArgs a, int slots) {
     constexpr int BM = 32 * NW, KD = D / 16, ND = D / 32, RB = 2 * D;  // RB: bytes of a row
@@ -1070,9 +1079,12 @@ __global__ __launch_bounds__(256) void k_attn_join(const JoinArgs a) {
 // Query rows of a k_attn_rows workgroup. D = 256: four waves, whose registers the CU's whole file holds (16 query and 2 K/V
 // heads, 3,000 tokens: 113 us; eight waves with tiles of 32 positions 207, 16 over 8 heads and 8,000 tokens 598 and 582).
 // D = 128: eight.
-// D = 64, where a tile's weights cost twice its matrix products: four waves, four workgroups to a CU,
-// where there are enough to keep them all busy (64 query and 8 K/V heads, 4,000 tokens: 164 -> 150 us; 1,500 in three
-// prompts: 28.4 -> 26.3), else eight waves that take turns (1,018 tokens behind 24,000: 399 us, 428 with four).
+// D = 64, where a tile's weights cost twice its matrix products: four waves, four workgroups to a CU, where there are enough
+// to keep them all busy, else eight waves that take turns. 64 query and 8 K/V heads, four and eight waves: 1,280 tokens, the
+// rule's border, 29.7 and 30.9 us alone, 76 and 92 behind 2,000 positions, 646 and 823 behind 24,000; 4,000 tokens 151 and 166,
+// 288 and 305, 1,817 and 1,821; 2,000 tokens behind 24,000 912 and 883. Below it, behind 24,000, 1,000 tokens 482 and 441, 300
+// tokens 364 and 182. Without such a context four waves are ahead there, too (1,000 tokens 23.9 and 25.9, and far where eight
+// leave tiles few enough to be cut in parts: 300 tokens 11 and 39), but how long the context is only the device knows.
 int rows_of(int d, int64_t rows, int hk) { return d == 256 || (d == 64 && rows / 128 * hk >= 640) ? 128 : 256; }
 
 template <bool F16>
@@ -1114,6 +1126,10 @@ int row_parts(int64_t groups, int64_t positions) {
 
 // Whether k_attn_flat takes each sequence whole, which spares the records and k_attn_join: where no table holds more than
 // 4 steps of positions, or 8 where there are workgroups enough without pieces, or a prefix's records to be added anyway.
+// Whole and in pieces, 4 K/V heads of 128, every sequence as long as its table: one sequence of 512 positions 7.6 and 8.9 us, 768
+// 9.1 and 9.4, 1,024 10.8 and 9.5; 64 of 512 14.2 and 18.7, of 1,024 23.6 and 27.6. Behind a prefix of 2,000: one of 512 17.1
+// and 17.2, of 1,024 20.4 and 17.7 (the loss at few sequences); 16 of 1,024 24.2 and 24.7, 64 43.0 and 46.8. Longer tables gain,
+// too, where all are full (64 of 2,048: 43.0 and 47.0), but one long sequence among short ones would then be the call.
 bool takes_whole(int B, int hq, int hk, int64_t positions, bool prefix) {
     const int64_t groups = (int64_t)B * hk * ((hq / hk + 15) / 16);
     return positions <= (groups >= 256 || prefix ? 8 : 4) * kStep;
