@@ -215,3 +215,10 @@ def test_strides_of_dimensions_of_size_one_say_nothing():
     assert kernels._paged_cache(q, *one_head, table, "t")[4][4:] == (8192, 0, 128)
     with pytest.raises(AssertionError):
         kernels._paged_cache(q, one_head[0], x.as_strided((3, 1, 64, 128), (8704, 8192, 136, 1)), table, "t")
+
+
+def test_a_cache_without_heads_is_refused():
+    kc = torch.zeros(4, 0, 16, 64, dtype=torch.bfloat16)
+    with pytest.raises(AssertionError, match="K/V heads"):
+        kernels.attn_batch(torch.zeros(2, 8, 64, dtype=torch.bfloat16), kc, kc, torch.zeros(2, dtype=torch.int32),
+                           torch.zeros(2, 1, dtype=torch.int32), 0.1)

@@ -564,7 +564,7 @@ def _paged_cache(q, kc, vc, table, what):
     if P == 1 or hk == 1:  # the stride of a dimension of size 1 says nothing
         st, sv = (tuple(0 if n == 1 else x for n, x in zip(shape, s)) for s in (st, sv))
     assert st[3] == 1 and st == sv, "caches need contiguous rows and equal strides"
-    assert hq % hk == 0, f"{hq} query heads over {hk} K/V heads"
+    assert hk >= 1 and hq % hk == 0, f"{hq} query heads over {hk} K/V heads"
     if table.dtype != torch.int32 or table.dim() != 2 or not table.is_contiguous():
         raise TypeError("table must be a contiguous int32 [B, pages of a sequence] tensor")
     B, width = table.shape
